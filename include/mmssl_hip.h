@@ -729,6 +729,30 @@ int mmssl_peer_pull_sum_rows_f32(mmssl_peer* p, int win_id, int64_t row0, int64_
 int mmssl_peer_sum_slots_f32(const float* slots, int n, int64_t stride, int64_t len, float* out, void* stream);
 int mmssl_peer_error(mmssl_peer* p, uint32_t* err);
 
+/* ------------------------------------------------------------------------------------
+ * Operators of a full-catalogue softmax model (no reference call site: what a sequence or full-softmax model trained next
+ * to the tables above needs). They take fp32, bf16 and fp16: `dtype` below is one of these codes, strides (ld*) are in
+ * elements, base pointers need the alignment of one element only. Sums, softmax statistics and means are held in 32 bits or
+ * more and every output is rounded once, to nearest even. Results do not depend on the order in which blocks run.
+ * ---------------------------------------------------------------------------------- */
+#define MMSSL_F32  0
+#define MMSSL_BF16 1
+#define MMSSL_F16  2
+
+/* Row lookup with scaling (csrc/embed.hip): out[i, :] = scale * table[idx[i], :] for n tokens; idx is int32 (idx_bytes 4) or
+ * int64 (8); table row r starts at table + r * ldt, output row i at out + i * ldo. A token equal to padding_idx (only with
+ * has_padding; any number, in the table or not) gives a row of zeros, any other token outside [0, rows) a row of NaN;
+ * neither reads the table. rows <= 2^31 - 2, n <= 2^31 - 16, d <= 2^24. */
+int mmssl_embed_rows(const void* table, int64_t ldt, int dtype, int64_t rows, int d, const void* idx, int idx_bytes,
+                     int64_t n, float scale, int has_padding, int64_t padding_idx, void* out, int64_t ldo, void* stream);
+/* Its gradient: grad[v, :] = scale * (sum of g[i, :] over the places i with idx[i] == v, fp32, in a fixed order), every one
+ * of the [rows, d] entries written (rows without a token as zeros); padding and out-of-range tokens add nothing. g row i
+ * starts at g + i * ldg (ldg = 0: one row for all). The workspace (16-byte aligned) need not be cleared. */
+size_t mmssl_embed_rows_bwd_workspace_bytes(int64_t rows, int d, int64_t n);
+int mmssl_embed_rows_bwd(const void* g, int64_t ldg, int dtype, const void* idx, int idx_bytes, int64_t n, int64_t rows, int d,
+                         float scale, int has_padding, int64_t padding_idx, void* grad, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -229,6 +229,11 @@ SIGNATURES = {
     "mmssl_bpr_bwd_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                   c_int, c_float, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                   c_void_p, c_void_p]),
+    "mmssl_embed_rows": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_void_p, c_int, c_int64, c_float, c_int, c_int64,
+                                 c_void_p, c_int64, c_void_p]),
+    "mmssl_embed_rows_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64]),
+    "mmssl_embed_rows_bwd": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_int, c_float, c_int,
+                                     c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -1405,3 +1405,105 @@ class _NGCFCombine(torch.autograd.Function):
 
 def ngcf_combine(G, B, keep=None, scale=1.0):
     return _NGCFCombine.apply(G, B, keep, scale)
+
+
+# ---------------------------------------------------------------------------------------
+# Operators of a full-catalogue softmax model (csrc/embed.hip, layernorm.hip, logprobs.hip): fp32, bf16 and fp16
+# ---------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # MMSSL_F32 / BF16 / F16
+
+
+def _typed(t, name):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise _lib.MmsslError("%s must be a CUDA (HIP) tensor: this package has no CPU path" % name)
+    if t.dtype not in _DTYPES:
+        raise _lib.MmsslError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return _DTYPES[t.dtype]
+
+
+def _same_device(t, other, name):
+    if other.device != t.device:
+        raise _lib.MmsslError("%s is on %s, expected %s" % (name, other.device, t.device))
+
+
+def _rows2d(t):
+    """(t as [rows, d] with unit column stride, row pitch): a view where the strides allow it."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _call(name, t, *args):
+    """One C entry point on the current stream of t's device, whichever device is current."""
+    dev = t.device.index
+    fn = getattr(_lib.lib(), name)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _tokens(idx, name, device):
+    """int32 / int64 numbers on `device`, contiguous (lists and host tensors are uploaded like ops._idx does)."""
+    if not isinstance(idx, torch.Tensor):
+        idx = torch.as_tensor(idx)
+        if idx.numel() == 0:
+            idx = idx.to(torch.int64)
+    if idx.dtype not in (torch.int64, torch.int32):
+        raise _lib.MmsslError("%s must hold int64 or int32 numbers, got %s" % (name, idx.dtype))
+    if idx.device != device:
+        if idx.is_cuda:
+            raise _lib.MmsslError("%s is on %s, expected %s" % (name, idx.device, device))
+        idx = idx.to(device)
+    return idx if idx.is_contiguous() else idx.contiguous()
+
+
+def _embed_fwd(table, idx, scale, pad):
+    rows, d = table.shape
+    out = torch.empty(idx.shape + (d,), dtype=table.dtype, device=table.device)
+    ldt = table.stride(0) if rows > 1 else d
+    _call("mmssl_embed_rows", table, table.data_ptr(), ldt, _DTYPES[table.dtype], rows, d, idx.data_ptr(), idx.element_size(),
+          idx.numel(), scale, pad is not None, pad or 0, out.data_ptr(), d)
+    return out
+
+
+class _EmbedRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, idx, scale, pad):
+        ctx.save_for_backward(idx)
+        ctx.cfg = (table.shape, scale, pad)
+        return _embed_fwd(table, idx, scale, pad)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (idx,) = ctx.saved_tensors
+        (rows, d), scale, pad = ctx.cfg
+        g, ldg = _rows2d(g)
+        grad = torch.empty((rows, d), dtype=g.dtype, device=g.device)
+        nb = _lib.lib().mmssl_embed_rows_bwd_workspace_bytes(rows, d, idx.numel())
+        ws = torch.empty(nb, dtype=torch.uint8, device=g.device)
+        _call("mmssl_embed_rows_bwd", g, g.data_ptr(), ldg, _DTYPES[g.dtype], idx.data_ptr(), idx.element_size(), idx.numel(),
+              rows, d, scale, pad is not None, pad or 0, grad.data_ptr(), ws.data_ptr(), nb)
+        return grad, None, None, None
+
+
+def embed_rows(table, idx, scale=1.0, padding_idx=None):
+    """scale * table[idx]: rows of an embedding table [rows, d] for tokens of any shape (int64 or int32), fp32 / bf16 / fp16,
+    rounded once. `padding_idx`: tokens of this number (in the table or not, e.g. the -1 that topk_rows pads with) give rows
+    of zeros; any other token outside the table gives a row of NaN. Differentiable in `table`: the dense [rows, d] gradient
+    adds equal tokens in the order of their places with fp32 sums (the same call gives the same bits); padding and tokens
+    outside the table add nothing."""
+    _typed(table, "table")
+    if table.dim() != 2 or table.shape[1] < 1 or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise _lib.MmsslError("embed_rows: table must be [rows, d] with unit column stride")
+    idx = _tokens(idx, "idx", table.device)
+    pad = None if padding_idx is None else int(padding_idx)
+    if table.requires_grad and torch.is_grad_enabled():
+        return _EmbedRows.apply(table, idx, float(scale), pad)
+    return _embed_fwd(table, idx, float(scale), pad)
