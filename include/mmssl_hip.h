@@ -753,6 +753,20 @@ int mmssl_embed_rows_bwd(const void* g, int64_t ldg, int dtype, const void* idx,
                          float scale, int has_padding, int64_t padding_idx, void* grad, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* Layer norm over the rows of X [rows, d] (csrc/layernorm.hip): Y = (x - mean) / sqrt(var + eps) * weight + bias, var the mean
+ * square around the mean. X row r starts at X + r * ldx (ldx = 0: one row for all), Y is contiguous. weight and bias (either
+ * may be NULL: 1 and 0) hold d numbers of type param_dtype. stats (may be NULL): [rows][2] fp32, mean and 1 / sqrt(var + eps)
+ * of each row, for the backward pass. d <= 2^24. */
+int mmssl_layernorm_rows(const void* X, int64_t ldx, int dtype, int64_t rows, int d, const void* weight, const void* bias,
+                         int param_dtype, float eps, void* Y, float* stats, void* stream);
+/* Its gradients: GX [rows, d] contiguous, gweight and gbias [d] of type param_dtype, each of which may be NULL (not wanted).
+ * The sums over the rows are fp32 in a fixed order; rows = 0 writes zeros. The workspace (16-byte aligned, wanted only with
+ * gweight or gbias) need not be cleared. */
+size_t mmssl_layernorm_rows_bwd_workspace_bytes(int dtype, int64_t rows, int d);
+int mmssl_layernorm_rows_bwd(const void* X, int64_t ldx, const void* G, int64_t ldg, int dtype, int64_t rows, int d,
+                             const void* weight, int param_dtype, const float* stats, void* GX, void* gweight, void* gbias,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

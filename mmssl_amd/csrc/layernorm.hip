@@ -1,0 +1,543 @@
+// Layer norm over the rows of X [rows, d], its backward pass and the gradients of weight and bias.
+//
+//   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) r, y = h w + b
+//   gx = r (q - mean(q) - h mean(q h)),  q = gy w;      gw = sum over rows of gy h,  gb = sum over rows of gy
+//
+// All three directions stream their operands once: a row lives in the registers of a lane group (up to 16 values a lane;
+// the variance is taken around the mean in a second sweep over the registers, so nothing cancels), the columns a lane holds
+// are the same for every row, so the weight stays in registers and the weight's gradient adds up there over the rows of a
+// block; the blocks' partial sums meet in a second launch in a fixed order. Rows longer than 16384 are swept from memory.
+#include <algorithm>
+
+#include "typed.hpp"
+
+using namespace mmssl;
+
+namespace {
+
+constexpr int kMaxInRegs = 16384;
+
+// LPR lanes a row (a power of two; above 64 whole waves of one block), NV vectors a lane: vector v of lane l holds the
+// columns [(v * LPR + l) * N, + N)
+template <class T, int LPR, int NV, bool FULL>
+struct RowTile {
+  static constexpr int N = Vec<T>::N;
+  static constexpr int TPB = LPR > kBlock ? LPR : kBlock;
+  static constexpr int GPB = TPB / LPR;          // rows of a block at a time
+  static constexpr int WPR = LPR > 64 ? LPR / 64 : 1;
+  typedef typename Vec<T>::f32 F;
+  typedef typename Vec<T>::raw R;
+
+  __device__ static __forceinline__ int col(int v, int lig) { return (v * LPR + lig) * N; }
+
+  __device__ static __forceinline__ void load(const T* __restrict__ p, int d, int lig, R (&x)[NV]) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = col(v, lig);
+      x[v] = (typename Vec<T>::raw)(T)0.0f;
+      if (c < d) x[v] = load_raw<T, FULL>(p + c, d - c);
+    }
+  }
+};
+
+// a weight / bias vector of type code dt as fp32, columns behind the row as 0
+template <int N>
+__device__ __forceinline__ void load_param(const void* __restrict__ w, int dt, int c, int d, float* out) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    float f = 0.f;
+    if (c + k < d) {
+      if (dt == MMSSL_F32) f = static_cast<const float*>(w)[c + k];
+      else if (dt == MMSSL_BF16) f = (float)static_cast<const bf16_t*>(w)[c + k];
+      else f = (float)static_cast<const f16_t*>(w)[c + k];
+    }
+    out[k] = f;
+  }
+}
+
+// Sums of NS values over the LPR lanes of a row; every lane ends with them. `red` = two copies of [NS][waves]: used in turn,
+// one barrier a call is enough.
+template <int LPR, int NS>
+__device__ __forceinline__ void row_sum(float (&s)[NS], float* red, int& turn) {
+#pragma unroll
+  for (int k = 0; k < NS; ++k) s[k] = group_sum<(LPR < 64 ? LPR : 64)>(s[k]);
+  if (LPR > 64) {
+    constexpr int W = LPR / 64;
+    float* r = red + turn * (NS * W);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < NS; ++k) r[k * W + (threadIdx.x >> 6)] = s[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      float a = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) a += r[k * W + w];
+      s[k] = a;
+    }
+  }
+}
+
+template <class T, int LPR, int NV, bool FULL>
+__global__ __launch_bounds__((RowTile<T, LPR, NV, FULL>::TPB)) void ln_fwd_kernel(const T* __restrict__ X, int64_t ldx,
+                                                                                  int64_t rows, int d,
+                                                                                  const void* __restrict__ w,
+                                                                                  const void* __restrict__ b, int pdt,
+                                                                                  float eps, T* __restrict__ Y,
+                                                                                  float2* __restrict__ stats) {
+  typedef RowTile<T, LPR, NV, FULL> Q;
+  constexpr int N = Q::N;
+  __shared__ float red[2 * Q::WPR];
+  int turn = 0;
+  const int lig = threadIdx.x & (LPR - 1);
+  const int64_t step = (int64_t)gridDim.x * Q::GPB;
+  const float inv_d = 1.0f / (float)d;
+  float W[NV][N], Bb[NV][N];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = Q::col(v, lig);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      W[v][k] = 1.f;
+      Bb[v][k] = 0.f;
+    }
+    if (w) load_param<N>(w, pdt, c, d, W[v]);
+    if (b) load_param<N>(b, pdt, c, d, Bb[v]);
+  }
+  int64_t row = (int64_t)blockIdx.x * Q::GPB + threadIdx.x / LPR;
+  typename Q::R raw[NV];
+  if (row < rows) Q::load(X + row * ldx, d, lig, raw);
+  for (; row < rows; row += step) {
+    typename Q::F x[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) x[v] = to_f32<T>(raw[v]);
+    if (row + step < rows) Q::load(X + (row + step) * ldx, d, lig, raw);      // the next row, under this one's sums
+    float s[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) s[0] += x[v][k];
+    row_sum<LPR, 1>(s, red, turn);
+    const float mu = s[0] / (float)d;        // the mean itself, not its product with a rounded 1 / d: x - mu may cancel
+    float q[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float t = Q::col(v, lig) + (FULL ? 0 : k) < d ? x[v][k] - mu : 0.f;
+        x[v][k] = t;
+        q[0] += t * t;
+      }
+    row_sum<LPR, 1>(q, red, turn);
+    const float r = 1.0f / sqrtf(q[0] * inv_d + eps);
+    if (stats && lig == 0) stats[row] = make_float2(mu, r);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = Q::col(v, lig);
+      typename Q::F y;
+#pragma unroll
+      for (int k = 0; k < N; ++k) y[k] = fmaf(x[v][k] * r, W[v][k], Bb[v][k]);
+      if (c < d) store_f32<T, FULL>(Y + row * d + c, d - c, y);
+    }
+  }
+}
+
+// part [blocks][2][d]: this block's sums of gy h and gy (NULL: not wanted); GX may be NULL
+template <class T, int LPR, int NV, bool FULL>
+__global__ __launch_bounds__((RowTile<T, LPR, NV, FULL>::TPB)) void ln_bwd_kernel(
+    const T* __restrict__ X, int64_t ldx, const T* __restrict__ G, int64_t ldg, int64_t rows, int d,
+    const void* __restrict__ w, int pdt, const float2* __restrict__ stats, T* __restrict__ GX, float* __restrict__ part) {
+  typedef RowTile<T, LPR, NV, FULL> Q;
+  constexpr int N = Q::N;
+  __shared__ float red[4 * Q::WPR];
+  int turn = 0;
+  const int lig = threadIdx.x & (LPR - 1);
+  const int64_t step = (int64_t)gridDim.x * Q::GPB;
+  const float inv_d = 1.0f / (float)d;
+  float W[NV][N], aw[NV][N], ab[NV][N];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) W[v][k] = 1.f, aw[v][k] = 0.f, ab[v][k] = 0.f;
+    if (w) load_param<N>(w, pdt, Q::col(v, lig), d, W[v]);
+  }
+  int64_t row = (int64_t)blockIdx.x * Q::GPB + threadIdx.x / LPR;
+  typename Q::R rx[NV], rg[NV];
+  if (row < rows) {
+    Q::load(X + row * ldx, d, lig, rx);
+    Q::load(G + row * ldg, d, lig, rg);
+  }
+  for (; row < rows; row += step) {
+    typename Q::F x[NV], g[NV];
+    const float2 st = stats[row];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      x[v] = to_f32<T>(rx[v]);
+      g[v] = to_f32<T>(rg[v]);
+    }
+    if (row + step < rows) {
+      Q::load(X + (row + step) * ldx, d, lig, rx);
+      Q::load(G + (row + step) * ldg, d, lig, rg);
+    }
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float h = (x[v][k] - st.x) * st.y;           // columns behind the row: g = 0, so every product is
+        const float gg = g[v][k], q = gg * W[v][k];
+        x[v][k] = h;
+        aw[v][k] = fmaf(gg, h, aw[v][k]);
+        ab[v][k] += gg;
+        g[v][k] = q;
+        s[0] += q;
+        s[1] = fmaf(q, h, s[1]);
+      }
+    if (!GX) continue;                                     // uniform
+    row_sum<LPR, 2>(s, red, turn);
+    const float m1 = s[0] * inv_d, m2 = s[1] * inv_d;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = Q::col(v, lig);
+      typename Q::F y;
+#pragma unroll
+      for (int k = 0; k < N; ++k) y[k] = st.y * (g[v][k] - m1 - x[v][k] * m2);
+      if (c < d) store_f32<T, FULL>(GX + row * d + c, d - c, y);
+    }
+  }
+  if (!part) return;
+  // the groups of a block, in their order
+  float* out = part + (int64_t)blockIdx.x * 2 * d;
+  if (Q::GPB == 1) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int c = Q::col(v, lig) + k;
+        if (c < d) {
+          out[c] = aw[v][k];
+          out[d + c] = ab[v][k];
+        }
+      }
+    return;
+  }
+  constexpr int kSlots = Q::TPB * N;              // one vector of every lane at a time
+  __shared__ float slot[Q::GPB == 1 ? 1 : 2 * kSlots];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      slot[threadIdx.x * N + k] = aw[v][k];
+      slot[kSlots + threadIdx.x * N + k] = ab[v][k];
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < 2 * LPR * N; j += Q::TPB) {
+      const int half = j / (LPR * N), at = j % (LPR * N);
+      float a = 0.f;
+#pragma unroll 4
+      for (int gidx = 0; gidx < Q::GPB; ++gidx) a += slot[half * kSlots + gidx * LPR * N + at];
+      const int c = v * LPR * N + at;
+      if (c < d) out[half * d + c] = a;
+    }
+  }
+}
+
+// gw / gb from the blocks' partial sums: 64 columns a block, its 16 groups of 16 lanes take a stripe of the partials each
+__global__ __launch_bounds__(kBlock) void ln_param_kernel(const float* __restrict__ part, int nparts, int d,
+                                                          void* __restrict__ gw, void* __restrict__ gb, int pdt) {
+  __shared__ float4 red[16][16];
+  const int l = threadIdx.x & 15, gidx = threadIdx.x >> 4;
+  const int64_t width = 2 * (int64_t)d;
+  const int64_t c = (int64_t)blockIdx.x * 64 + l * 4;
+  Vec<float>::f32 a = 0.f;
+  if (c < width) {
+#pragma unroll 4
+    for (int p = gidx; p < nparts; p += 16)
+      a += load_raw<float>(part + (int64_t)p * width + c, (int)min((int64_t)4, width - c));
+  }
+  red[gidx][l] = make_float4(a[0], a[1], a[2], a[3]);
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int64_t col = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += reinterpret_cast<const float*>(red[k])[threadIdx.x];
+    if (col < width) {
+      void* out = col < d ? gw : gb;
+      const int64_t j = col < d ? col : col - d;
+      if (out) {
+        if (pdt == MMSSL_F32) static_cast<float*>(out)[j] = t;
+        else if (pdt == MMSSL_BF16) static_cast<bf16_t*>(out)[j] = (bf16_t)t;
+        else static_cast<f16_t*>(out)[j] = (f16_t)t;
+      }
+    }
+  }
+}
+
+// ---- rows longer than the registers of a block hold: one block a row, three sweeps (the later ones from the caches) -------
+constexpr int kWideThreads = 1024;
+
+template <class T>
+__global__ __launch_bounds__(kWideThreads) void ln_fwd_wide_kernel(const T* __restrict__ X, int64_t ldx, int d,
+                                                                   const void* __restrict__ w, const void* __restrict__ b,
+                                                                   int pdt, float eps, T* __restrict__ Y,
+                                                                   float2* __restrict__ stats) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float red[2 * (kWideThreads / 64)];
+  int turn = 0;
+  const T* x = X + (int64_t)blockIdx.x * ldx;
+  T* y = Y + (int64_t)blockIdx.x * d;
+  const float inv_d = 1.0f / (float)d;
+  float s[1] = {0.f};
+  for (int c = threadIdx.x * N; c < d; c += kWideThreads * N) {
+    const typename Vec<T>::f32 f = to_f32<T>(load_raw<T>(x + c, d - c));
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[0] += f[k];
+  }
+  row_sum<kWideThreads, 1>(s, red, turn);
+  const float mu = s[0] / (float)d;        // the mean itself, not its product with a rounded 1 / d: x - mu may cancel
+  float q[1] = {0.f};
+  for (int c = threadIdx.x * N; c < d; c += kWideThreads * N) {
+    const typename Vec<T>::f32 f = to_f32<T>(load_raw<T>(x + c, d - c));
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float t = c + k < d ? f[k] - mu : 0.f;
+      q[0] += t * t;
+    }
+  }
+  row_sum<kWideThreads, 1>(q, red, turn);
+  const float r = 1.0f / sqrtf(q[0] * inv_d + eps);
+  if (stats && threadIdx.x == 0) stats[blockIdx.x] = make_float2(mu, r);
+  for (int c = threadIdx.x * N; c < d; c += kWideThreads * N) {
+    typename Vec<T>::f32 f = to_f32<T>(load_raw<T>(x + c, d - c));
+    float W[N], Bb[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) W[k] = 1.f, Bb[k] = 0.f;
+    if (w) load_param<N>(w, pdt, c, d, W);
+    if (b) load_param<N>(b, pdt, c, d, Bb);
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] = fmaf((f[k] - mu) * r, W[k], Bb[k]);
+    store_f32<T>(y + c, d - c, f);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(kWideThreads) void ln_gx_wide_kernel(const T* __restrict__ X, int64_t ldx,
+                                                                  const T* __restrict__ G, int64_t ldg, int d,
+                                                                  const void* __restrict__ w, int pdt,
+                                                                  const float2* __restrict__ stats, T* __restrict__ GX) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float red[4 * (kWideThreads / 64)];
+  int turn = 0;
+  const T* x = X + (int64_t)blockIdx.x * ldx;
+  const T* g = G + (int64_t)blockIdx.x * ldg;
+  T* gx = GX + (int64_t)blockIdx.x * d;
+  const float2 st = stats[blockIdx.x];
+  const float inv_d = 1.0f / (float)d;
+  float s[2] = {0.f, 0.f};
+#pragma unroll 1
+  for (int sweep = 0; sweep < 2; ++sweep) {
+    for (int c = threadIdx.x * N; c < d; c += kWideThreads * N) {
+      const typename Vec<T>::f32 xf = to_f32<T>(load_raw<T>(x + c, d - c)), gf = to_f32<T>(load_raw<T>(g + c, d - c));
+      float W[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) W[k] = 1.f;
+      if (w) load_param<N>(w, pdt, c, d, W);
+      typename Vec<T>::f32 o;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float h = (xf[k] - st.x) * st.y, q = gf[k] * W[k];
+        if (sweep == 0) {
+          s[0] += q;
+          s[1] = fmaf(q, h, s[1]);
+        }
+        o[k] = st.y * (q - s[0] - h * s[1]);
+      }
+      if (sweep) store_f32<T>(gx + c, d - c, o);
+    }
+    if (sweep == 0) {
+      row_sum<kWideThreads, 2>(s, red, turn);
+      s[0] *= inv_d;
+      s[1] *= inv_d;
+    }
+  }
+}
+
+// blockIdx.x: column tile of kBlock vectors; blockIdx.y: stripe of rows
+template <class T>
+__global__ __launch_bounds__(kBlock) void ln_gw_wide_kernel(const T* __restrict__ X, int64_t ldx, const T* __restrict__ G,
+                                                            int64_t ldg, int64_t rows, int d,
+                                                            const float2* __restrict__ stats, float* __restrict__ part) {
+  constexpr int N = Vec<T>::N;
+  const int c = (blockIdx.x * kBlock + threadIdx.x) * N;
+  if (c >= d) return;
+  typename Vec<T>::f32 aw = 0.f, ab = 0.f;
+#pragma unroll 2
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const typename Vec<T>::f32 x = to_f32<T>(load_raw<T>(X + r * ldx + c, d - c));
+    const typename Vec<T>::f32 g = to_f32<T>(load_raw<T>(G + r * ldg + c, d - c));
+    const float2 st = stats[r];
+    aw += g * ((x - st.x) * st.y);
+    ab += g;
+  }
+  float* out = part + (int64_t)blockIdx.y * 2 * d;
+  store_part<N>(out + c, d - c, aw);
+  store_part<N>(out + d + c, d - c, ab);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+struct Shape {
+  int lpr, nv;      // lpr 0: wide
+};
+
+// up to 16 values a lane (NV vectors of 16 bytes); the fewest lanes that hold the row, no fewer than 8
+Shape shape_for(int d, int es) {
+  const int n = 16 / es, vecs = (d + n - 1) / n, most = 16 / n;      // most = vectors a lane may hold: 4 (fp32), 2
+  if (d > kMaxInRegs) return {0, 0};
+  static const int lanes[] = {8, 16, 32, 64, 256, 1024};
+  for (int l : lanes) {
+    if (vecs <= l) return {l, 1};
+    if (l >= 64)
+      for (int nv = 2; nv <= most; nv *= 2)
+        if (vecs <= l * nv) return {l, nv};
+  }
+  return {0, 0};
+}
+
+int gpb_of(Shape q) { return q.lpr > kBlock ? 1 : kBlock / q.lpr; }
+
+// blocks of a launch over rows: enough to fill the chip (256 CUs) `per_cu` times, no more than the rows need
+int64_t blocks_for(int64_t rows, Shape q, int64_t most) { return std::min((rows + gpb_of(q) - 1) / gpb_of(q), most); }
+
+constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 1024;
+int64_t wide_stripes(int64_t rows) { return std::min<int64_t>(rows, 256); }
+int64_t parts_for(int64_t rows, int d, int es) {
+  const Shape q = shape_for(d, es);
+  return q.lpr ? blocks_for(rows, q, q.lpr > kBlock ? kBwdBlocks / 2 : kBwdBlocks) : wide_stripes(rows);
+}
+
+int check_common(int dtype, int64_t rows, int d, int pdt, float eps) {
+  if (!known_dtype(dtype) || !known_dtype(pdt) || rows < 0 || d < 1 || !(eps >= 0.f)) return MMSSL_E_BADARG;
+  // one block a row where rows are wide; a row's columns are counted in 32 bits
+  if (d > (1 << 24) || (d > kMaxInRegs && rows > 0x7fffffff)) return MMSSL_E_UNSUPP;
+  return 0;
+}
+
+#define LN_SHAPES(T, CALL)                            \
+  do {                                                \
+    const bool full = d % Vec<T>::N == 0;             \
+    if (q.lpr == 8) { CALL(T, 8, 1); }                \
+    else if (q.lpr == 16) { CALL(T, 16, 1); }         \
+    else if (q.lpr == 32) { CALL(T, 32, 1); }         \
+    else if (q.lpr == 64 && q.nv == 1) { CALL(T, 64, 1); }   \
+    else if (q.lpr == 64 && q.nv == 2) { CALL(T, 64, 2); }   \
+    else if (q.lpr == 64) { CALL(T, 64, 4); }                \
+    else if (q.lpr == 256 && q.nv == 1) { CALL(T, 256, 1); } \
+    else if (q.lpr == 256 && q.nv == 2) { CALL(T, 256, 2); } \
+    else if (q.lpr == 256) { CALL(T, 256, 4); }              \
+    else if (q.nv == 1) { CALL(T, 1024, 1); }                \
+    else if (q.nv == 2) { CALL(T, 1024, 2); }                \
+    else { CALL(T, 1024, 4); }                               \
+  } while (0)
+
+}  // namespace
+
+extern "C" int mmssl_layernorm_rows(const void* X, int64_t ldx, int dtype, int64_t rows, int d, const void* weight,
+                                    const void* bias, int param_dtype, float eps, void* Y, float* stats, void* stream) {
+  if (int rc = check_common(dtype, rows, d, param_dtype, eps)) return rc;
+  if (rows == 0) return 0;
+  const size_t es = dtype_bytes(dtype), ps = dtype_bytes(param_dtype);
+  if (!X || !Y || ldx < 0 || !aligned_to(X, es) || !aligned_to(Y, es) || !aligned_to(weight, ps) || !aligned_to(bias, ps) ||
+      !aligned_to(stats, 8))
+    return MMSSL_E_BADARG;
+  const hipStream_t s = as_stream(stream);
+  const Shape q = shape_for(d, (int)es);
+  if (!q.lpr) {
+#define LN_FWD_WIDE(T)                                                                                                   \
+  hipLaunchKernelGGL(ln_fwd_wide_kernel<T>, dim3((unsigned)rows), dim3(kWideThreads), 0, s, (const T*)X, ldx, d, weight,  \
+                     bias, param_dtype, eps, (T*)Y, (float2*)stats)
+    MMSSL_BY_DTYPE(dtype, LN_FWD_WIDE);
+    MMSSL_LAUNCH_CHECK();
+    return 0;
+  }
+  const dim3 grid((unsigned)blocks_for(rows, q, q.lpr > kBlock ? kFwdBlocks / 4 : kFwdBlocks));
+  const dim3 block(q.lpr > kBlock ? q.lpr : kBlock);
+#define LN_FWD_F(T, L, V, F)                                                                                             \
+  hipLaunchKernelGGL((ln_fwd_kernel<T, L, V, F>), grid, block, 0, s, (const T*)X, ldx, rows, d, weight, bias,             \
+                     param_dtype, eps, (T*)Y, (float2*)stats)
+#define LN_FWD_V(T, L, V)                                          \
+  if constexpr (V * Vec<T>::N <= 16) {                             \
+    if (full) LN_FWD_F(T, L, V, true);                             \
+    else LN_FWD_F(T, L, V, false);                                 \
+  }
+#define LN_FWD(T) LN_SHAPES(T, LN_FWD_V)
+  MMSSL_BY_DTYPE(dtype, LN_FWD);
+  MMSSL_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" size_t mmssl_layernorm_rows_bwd_workspace_bytes(int dtype, int64_t rows, int d) {
+  if (!known_dtype(dtype) || rows < 0 || d < 1 || d > (1 << 24)) return 0;
+  return (size_t)parts_for(rows, d, dtype_bytes(dtype)) * 2 * d * 4 + 16;
+}
+
+extern "C" int mmssl_layernorm_rows_bwd(const void* X, int64_t ldx, const void* G, int64_t ldg, int dtype, int64_t rows,
+                                        int d, const void* weight, int param_dtype, const float* stats, void* GX,
+                                        void* gweight, void* gbias, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+  if (int rc = check_common(dtype, rows, d, param_dtype, 0.f)) return rc;
+  const size_t es = dtype_bytes(dtype), ps = dtype_bytes(param_dtype);
+  const bool params = gweight || gbias;
+  if (ldx < 0 || ldg < 0 || !aligned_to(X, es) || !aligned_to(G, es) || !aligned_to(GX, es) || !aligned_to(weight, ps) ||
+      !aligned_to(gweight, ps) || !aligned_to(gbias, ps) || !aligned_to(stats, 8))
+    return MMSSL_E_BADARG;
+  if (rows > 0 && (!X || !G || !stats)) return MMSSL_E_BADARG;
+  if (!GX && !params) return 0;
+  float* part = static_cast<float*>(workspace);
+  if (params && (!workspace || !aligned_to(workspace, 16) ||
+                 workspace_bytes < mmssl_layernorm_rows_bwd_workspace_bytes(dtype, rows, d)))
+    return MMSSL_E_WORKSPACE;
+  const hipStream_t s = as_stream(stream);
+  const Shape q = shape_for(d, (int)es);
+  const int64_t nparts = parts_for(rows, d, (int)es);
+  if (rows > 0 && q.lpr) {
+    const dim3 grid((unsigned)nparts), block(q.lpr > kBlock ? q.lpr : kBlock);
+    float* pp = params ? part : nullptr;
+#define LN_BWD_F(T, L, V, F)                                                                                             \
+  hipLaunchKernelGGL((ln_bwd_kernel<T, L, V, F>), grid, block, 0, s, (const T*)X, ldx, (const T*)G, ldg, rows, d, weight, \
+                     param_dtype, (const float2*)stats, (T*)GX, pp)
+#define LN_BWD_V(T, L, V)                                          \
+  if constexpr (V * Vec<T>::N <= 16) {                             \
+    if (full) LN_BWD_F(T, L, V, true);                             \
+    else LN_BWD_F(T, L, V, false);                                 \
+  }
+#define LN_BWD(T) LN_SHAPES(T, LN_BWD_V)
+    MMSSL_BY_DTYPE(dtype, LN_BWD);
+    MMSSL_LAUNCH_CHECK();
+  } else if (rows > 0) {
+#define LN_GX_WIDE(T)                                                                                                    \
+  hipLaunchKernelGGL(ln_gx_wide_kernel<T>, dim3((unsigned)rows), dim3(kWideThreads), 0, s, (const T*)X, ldx, (const T*)G, \
+                     ldg, d, weight, param_dtype, (const float2*)stats, (T*)GX)
+#define LN_GW_WIDE(T)                                                                                                    \
+  hipLaunchKernelGGL(ln_gw_wide_kernel<T>, dim3((unsigned)((d + kBlock * Vec<T>::N - 1) / (kBlock * Vec<T>::N)),          \
+                                                (unsigned)nparts),                                                       \
+                     dim3(kBlock), 0, s, (const T*)X, ldx, (const T*)G, ldg, rows, d, (const float2*)stats, part)
+    if (GX) {
+      MMSSL_BY_DTYPE(dtype, LN_GX_WIDE);
+      MMSSL_LAUNCH_CHECK();
+    }
+    if (params) {
+      MMSSL_BY_DTYPE(dtype, LN_GW_WIDE);
+      MMSSL_LAUNCH_CHECK();
+    }
+  }
+  if (params) {
+    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)((2 * (int64_t)d + 63) / 64)), dim3(kBlock), 0, s,
+                       (const float*)part, (int)nparts, d, gweight, gbias, param_dtype);
+    MMSSL_LAUNCH_CHECK();
+  }
+  return 0;
+}

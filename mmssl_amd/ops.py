@@ -1507,3 +1507,70 @@ def embed_rows(table, idx, scale=1.0, padding_idx=None):
     if table.requires_grad and torch.is_grad_enabled():
         return _EmbedRows.apply(table, idx, float(scale), pad)
     return _embed_fwd(table, idx, float(scale), pad)
+
+
+def _layernorm_fwd(X, weight, bias, eps, want_stats):
+    X2, ldx = _rows2d(X)
+    rows, d = X2.shape
+    y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=X.device) if want_stats else None
+    p = weight if weight is not None else bias
+    _call("mmssl_layernorm_rows", X, X2.data_ptr(), ldx, _DTYPES[X.dtype], rows, d, _ptr(weight), _ptr(bias),
+          0 if p is None else _DTYPES[p.dtype], eps, y.data_ptr(), _ptr(stats))
+    return y, X2, stats
+
+
+class _LayerNormRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, X, weight, bias, eps):
+        y, X2, stats = _layernorm_fwd(X, weight, bias, eps, True)
+        ctx.save_for_backward(X2 if X.dim() != 2 else X, weight, stats)
+        ctx.cfg = (X.shape, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        X, weight, stats = ctx.saved_tensors
+        shape, bias_dtype = ctx.cfg
+        X2, ldx = _rows2d(X)
+        rows, d = X2.shape
+        g, ldg = _rows2d(g)
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        gx = torch.empty(shape, dtype=X2.dtype, device=X2.device) if want_x else None
+        pdt = weight.dtype if weight is not None else bias_dtype if bias_dtype is not None else X2.dtype
+        gw = torch.empty(d, dtype=pdt, device=X2.device) if want_w else None
+        gb = torch.empty(d, dtype=pdt, device=X2.device) if want_b else None
+        nb = _lib.lib().mmssl_layernorm_rows_bwd_workspace_bytes(_DTYPES[X2.dtype], rows, d) if want_w or want_b else 0
+        ws = torch.empty(nb, dtype=torch.uint8, device=X2.device) if nb else None
+        _call("mmssl_layernorm_rows_bwd", X2, X2.data_ptr(), ldx, g.data_ptr(), ldg, _DTYPES[X2.dtype], rows, d, _ptr(weight),
+              _DTYPES[pdt], stats.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nb)
+        return gx, gw, gb, None
+
+
+def layernorm_rows(X, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last dimension: (x - mean) / sqrt(var + eps) * weight + bias, fp32 / bf16 / fp16 with fp32 means
+    and variances, rounded once. `weight` / `bias`: [d] tensors of X's type or fp32 (both of one type), or None.
+    Differentiable in X, weight and bias; the parameters' sums over the rows are fp32 in a fixed order."""
+    _typed(X, "X")
+    if X.dim() < 1 or X.shape[-1] < 1:
+        raise _lib.MmsslError("layernorm_rows: X must be [..., d] with d >= 1")
+    if not 0.0 <= eps < float("inf"):
+        raise _lib.MmsslError("layernorm_rows: eps must be a finite number >= 0, got %r" % (eps,))
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        _typed(p, name)
+        _same_device(X, p, name)
+        if p.dim() != 1 or p.shape[0] != X.shape[-1]:
+            raise _lib.MmsslError("layernorm_rows: %s must be [%d], got %s" % (name, X.shape[-1], tuple(p.shape)))
+        if p.dtype != X.dtype and p.dtype != torch.float32:
+            raise _lib.MmsslError("layernorm_rows: %s must be %s or float32, got %s" % (name, X.dtype, p.dtype))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise _lib.MmsslError("layernorm_rows: weight and bias must be of one type")
+    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    if torch.is_grad_enabled() and (X.requires_grad or (w is not None and w.requires_grad)
+                                    or (b is not None and b.requires_grad)):
+        return _LayerNormRows.apply(X, w, b, float(eps))
+    return _layernorm_fwd(X, w, b, float(eps), False)[0]

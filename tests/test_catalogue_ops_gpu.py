@@ -162,3 +162,147 @@ def test_embed_gradient_where_places_times_width_pass_32_bits():
     want = torch.zeros(rows, dtype=torch.float32)
     want[7], want[9], want[49] = 8.0, 5.0, 2.0
     assert torch.equal(got.float().cpu(), want[:, None].expand(rows, d))
+
+
+# ---- layernorm_rows ---------------------------------------------------------------------------------------------------
+def norm_exact(x, w, b, eps, g):
+    """y, gx, gw, gb in 64 bits, and the sums of magnitudes behind the last two."""
+    x, g = x.double(), g.double()
+    d = x.shape[-1]
+    w1 = torch.ones(d, dtype=torch.float64) if w is None else w.double()
+    mu = x.mean(-1, keepdim=True)
+    var = ((x - mu) ** 2).mean(-1, keepdim=True)
+    r = 1 / (var + eps).sqrt()
+    h = (x - mu) * r
+    y = h * w1 + (0 if b is None else b.double())
+    q = g * w1
+    gx = r * (q - q.mean(-1, keepdim=True) - h * (q * h).mean(-1, keepdim=True))
+    flat = lambda t: t.reshape(-1, d)      # noqa: E731
+    # how far the 32-bit statistics let h be off: the mean by (d + 2) 2^-24 of the magnitudes' mean, the deviation's square by
+    # the same share again, and six roundings
+    e = (6 + d) * 2.0 ** -24
+    eh = e * (1 + 2 * x.abs().mean(-1, keepdim=True) * r) + h.abs() * e
+    qa = q.abs()
+    egx = r * (e * (qa + qa.mean(-1, keepdim=True) + h.abs() * (qa * h.abs()).mean(-1, keepdim=True)) * 3
+               + eh * (qa * h.abs()).mean(-1, keepdim=True) + h.abs() * (qa * eh).mean(-1, keepdim=True))
+    n = max(1, flat(x).shape[0])
+    gw, gb = flat(g * h).sum(0), flat(g).sum(0)
+    egw = flat(g.abs() * eh).sum(0) + flat((g * h).abs()).sum(0) * (n + 3) * 2.0 ** -24
+    egb = flat(g.abs()).sum(0) * (n + 3) * 2.0 ** -24
+    ey = eh * w1.abs() + y.abs() * 2.0 ** -23 + (h * w1).abs() * 2.0 ** -23
+    return (y, gx, gw, gb), (ey, egx, egw, egb)
+
+
+def check_norm(shape, t, pt=None, eps=1e-5, affine=(True, True), seed=0, x=None, offset=0.5):
+    from mmssl_amd import ops
+    pt = t if pt is None else pt
+    g0 = gen(seed)
+    x = (torch.randn(shape, generator=g0) * 2 + offset).to(t) if x is None else x
+    d = shape[-1]
+    w = (1 + 0.3 * torch.randn(d, generator=g0)).to(pt) if affine[0] else None
+    b = (0.3 * torch.randn(d, generator=g0)).to(pt) if affine[1] else None
+    g = torch.randn(shape, generator=g0).to(t)
+    want, off = norm_exact(x, w, b, eps, g)
+    leaves = [v.to(DEV).requires_grad_(True) if v is not None else None for v in (x, w, b)]
+    y = ops.layernorm_rows(*leaves, eps=eps)
+    ins = [v for v in leaves if v is not None]
+    grads = iter(torch.autograd.grad(y, ins, g.to(DEV)))
+    got = [y] + [next(grads) if v is not None else None for v in leaves]
+    for name, a, v, o, ty in zip(("y", "gx", "gw", "gb"), got, want, off, (t, t, pt, pt)):
+        if a is not None:
+            assert a.dtype == ty, name
+            tiny = torch.finfo(ty).smallest_normal * torch.finfo(ty).eps
+            within(a, v, v.abs() * half_step(ty) + o * (1 + half_step(ty)) + tiny, name)
+    with torch.no_grad():
+        assert torch.equal(ops.layernorm_rows(*leaves, eps=eps), y)
+    return got
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,d", [(1, 1), (3, 2), (1, 8), (5, 31), (17, 32), (64, 64), (33, 65), (7, 128), (9, 200), (5, 256),
+                                    (3, 257), (11, 512), (4, 513), (5, 1000), (3, 1024), (2, 1500), (3, 2048), (2, 2047),
+                                    (3, 4096), (2, 4100), (1, 5001), (2, 8192), (2, 12345), (2, 16384), (3, 16385),
+                                    (2, 20000)])
+def test_layernorm_rows_and_gradients(rows, d, t):
+    check_norm((rows, d), t, seed=d)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,d", [(5000, 16), (1025, 64), (2100, 130), (3001, 384), (1300, 1028), (600, 4608), (530, 16500)])
+def test_layernorm_gradients_of_many_rows(rows, d, t):
+    """More rows than blocks: the weights' sums add up over a block's rows, then over the blocks."""
+    a = check_norm((rows, d), t, seed=rows)
+    b = check_norm((rows, d), t, seed=rows)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)), "the same call, the same bits"
+
+
+def test_layernorm_parameters_types_and_absence():
+    for affine in ((True, False), (False, True), (False, False)):
+        for t in TYPES:
+            check_norm((37, 96), t, affine=affine, seed=3)
+            check_norm((3, 17000), t, affine=affine, seed=3)
+    for t in (torch.bfloat16, torch.float16):
+        check_norm((29, 100), t, pt=torch.float32, seed=4)
+        check_norm((2, 16400), t, pt=torch.float32, seed=4)
+    check_norm((4, 64), torch.float32, eps=0.0)
+    check_norm((2, 3, 5, 24), torch.float32)
+    check_norm((40,), torch.float32)
+
+
+def test_layernorm_values_far_from_zero_and_constant_rows():
+    """The variance is taken around the mean: a row far from zero keeps its digits, a constant row gives the bias."""
+    from mmssl_amd import ops
+    x = torch.randn(40, 256, generator=gen(1)) + 4096.0
+    check_norm((40, 256), torch.float32, x=x)
+    c = torch.full((3, 100), 7.0, device=DEV)
+    b = torch.randn(100, device=DEV)
+    assert torch.equal(ops.layernorm_rows(c, None, b), b.expand(3, 100))
+    for bad in (float("nan"), float("inf")):
+        x = torch.randn(5, 300, generator=gen(2))
+        x[3, 17] = bad
+        y = ops.layernorm_rows(x.to(DEV)).cpu()
+        assert bool(y[3].isnan().all()) and bool(y[[0, 1, 2, 4]].isfinite().all())
+
+
+def test_layernorm_strides_and_empty_inputs():
+    from mmssl_amd import ops
+    for t in TYPES:
+        wide = torch.randn(50, 91, generator=gen(4)).to(t).to(DEV)
+        g = torch.randn(50, 33, generator=gen(5)).to(t).to(DEV)
+        for x in (wide[:, 5:38], wide[::3, 1:34], wide.t()[:33].t(), wide[:1, :33].expand(50, 33)):
+            a = x.detach().requires_grad_(True)
+            c = x.detach().contiguous().requires_grad_(True)
+            ya, yc = ops.layernorm_rows(a), ops.layernorm_rows(c)
+            gg = g[:x.shape[0]]
+            assert torch.equal(ya, yc)
+            assert torch.equal(torch.autograd.grad(ya, a, gg)[0], torch.autograd.grad(yc, c, gg)[0])
+        one = torch.randn(33, generator=gen(6)).to(t).to(DEV).expand(50, 33)
+        y = ops.layernorm_rows(c)
+        assert torch.equal(torch.autograd.grad(y, c, one, retain_graph=True)[0],
+                           torch.autograd.grad(y, c, one.contiguous())[0])
+        w = torch.ones(8, dtype=t, device=DEV, requires_grad=True)
+        x = torch.zeros(0, 8, dtype=t, device=DEV, requires_grad=True)
+        y = ops.layernorm_rows(x, w, w)
+        gx, gw = torch.autograd.grad(y, (x, w), torch.zeros_like(y))
+        assert y.shape == gx.shape == (0, 8) and not bool(gw.any())
+
+
+def test_layernorm_gradient_against_differences():
+    """The gradient of a weighted sum against central differences of the 64-bit formula along a random direction."""
+    from mmssl_amd import ops
+    g0 = gen(8)
+    x, w, b, c = (torch.randn(s, generator=g0, dtype=torch.float64) for s in ((6, 40), (40,), (40,), (6, 40)))
+    f = lambda x, w, b: (norm_exact(x, w, b, 1e-5, x)[0][0] * c).sum()        # noqa: E731
+    leaves = [v.float().to(DEV).requires_grad_(True) for v in (x, w, b)]
+    grads = torch.autograd.grad((ops.layernorm_rows(*leaves) * c.float().to(DEV)).sum(), leaves)
+    x, w, b = (v.detach().cpu().double() for v in leaves)
+    for k, v in enumerate((x, w, b)):
+        u = torch.randn(v.shape, generator=g0, dtype=torch.float64)
+        e = 1e-5
+        args = [x, w, b]
+        hi, lo = list(args), list(args)
+        hi[k], lo[k] = v + e * u, v - e * u
+        slope = float((f(*hi) - f(*lo)) / (2 * e))
+        mine = float((grads[k].cpu().double() * u).sum())
+        # differences: e^2 of the third derivative and 1e-16 / e of rounding, both far below the 32-bit sums' share
+        assert abs(mine - slope) <= 1e-5 * float((grads[k].cpu().double().abs() * u.abs()).sum()) + 1e-6, (k, mine, slope)
