@@ -767,6 +767,25 @@ int mmssl_layernorm_rows_bwd(const void* X, int64_t ldx, const void* G, int64_t 
                              const void* weight, int param_dtype, const float* stats, void* GX, void* gweight, void* gbias,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* Log probabilities over score rows X [rows, cols] (csrc/logprobs.hip; row r starts at X + r * ldx) at a temperature > 0:
+ *   logp[r] = log softmax(X[r] / temperature)[target[r]], entropy[r] of that distribution (nats), and for k > 0 the k <= 128
+ *   largest columns in descending value, ties by ascending column (the order of mmssl_topk_rows_f32): top_idx, top_logp [rows, k].
+ * target: int32 (target_bytes 4) or int64 (8); a target equal to ignore_index gives logp 0, any other outside [0, cols) NaN.
+ * An entry of -inf has probability 0 (and -inf as its logp); a row of nothing else has entropy 0 and logp -inf. A NaN or
+ * +inf in a row makes its logp and entropy NaN; NaN ranks above +inf. stats (may be NULL): [rows][4] fp32, 16-byte aligned,
+ * for the backward pass. k <= cols <= 2^31 - 16. The workspace (16-byte aligned) need not be cleared. */
+size_t mmssl_logprobs_rows_workspace_bytes(int dtype, int64_t rows, int64_t cols, int k);
+int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_t rows, int64_t cols, const void* target,
+                        int target_bytes, int64_t ignore_index, int k, float temperature, float* logp, float* entropy,
+                        float* top_logp, int64_t* top_idx, float* stats, void* workspace, size_t workspace_bytes,
+                        void* stream);
+/* Its gradient GX [rows, cols] (contiguous, X's type) from the gradients of logp, entropy [rows] and top_logp [rows, k] (each
+ * may be NULL: 0). Ignored and out-of-range targets name no column; a row of nothing but -inf gets zeros. */
+int mmssl_logprobs_rows_bwd(const void* X, int64_t ldx, int dtype, int64_t rows, int64_t cols, const void* target,
+                            int target_bytes, int64_t ignore_index, int k, float temperature, const int64_t* top_idx,
+                            const float* stats, const float* glogp, const float* gentropy, const float* gtop, void* GX,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

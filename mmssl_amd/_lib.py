@@ -239,6 +239,11 @@ SIGNATURES = {
     "mmssl_layernorm_rows_bwd_workspace_bytes": (c_size_t, [c_int, c_int64, c_int]),
     "mmssl_layernorm_rows_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_void_p, c_int,
                                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mmssl_logprobs_rows_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int]),
+    "mmssl_logprobs_rows": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int, c_int64, c_int, c_float,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mmssl_logprobs_rows_bwd": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int, c_int64, c_int, c_float,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,574 @@
+// Log probabilities of given columns of score rows X [rows, cols], the rows' entropy, their k best columns, and the gradient.
+//
+//   z = x / T, lp_j = z_j - log sum exp(z);  logp = lp_target, H = -sum p_j lp_j, top = the k largest x (ties: lowest column)
+//   gx_j = (1/T) (g_target [j = target] + sum_i gtop_i [j = top_i] - p_j (g_target + sum_i gtop_i) - gH p_j (lp_j + H))
+//
+// Forward: one read of X. A block holds a slice of a row in its registers: the slice's maximum m, S = sum e_j and
+// A = sum e_j y_j with y_j = (x_j - m) / T, e_j = exp(y_j); slices join by S = sum S_i 2^(d_i), A = sum 2^(d_i) (A_i + d_i S_i)
+// with d_i the distance of the slice's maximum from the row's. H = log S - A / S: both parts are >= 0, nothing cancels.
+// The best columns come out of the same registers: a lower bound of the k-th largest value from the threads' maxima leaves
+// about 2 k candidates, which are ranked by counting.
+// Backward: one read of X, one write of gx.
+#include <algorithm>
+
+#include "typed.hpp"
+
+using namespace mmssl;
+
+namespace {
+
+constexpr int kTopMax = 128;          // most alternatives
+constexpr int kCand = 1024;           // candidates of a slice that are ranked by counting
+constexpr int kWaves = kBlock / 64;
+constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.4426950408889634074f;
+constexpr float kFar = -1.0e4f;       // exp2 of this is 0; stands for -inf where 0 * -inf has to be 0
+
+// a value's place in the order of values as a whole number: NaN above +inf, -0 equal to 0
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+  if (o == 0xffffffffu) return __builtin_nanf("");
+  return __uint_as_float((o >> 31) ? (o & 0x7fffffffu) : ~o);
+}
+// (value, column) as one number: larger is better, equal values by the lower column. Never 0 for a column.
+__device__ __forceinline__ uint64_t pair_of(float x, int64_t col) {
+  return ((uint64_t)order_of(x) << 32) | (uint64_t)(0xffffffffu - (uint32_t)col);
+}
+__device__ __forceinline__ int64_t col_of(uint64_t p) { return (int64_t)(0xffffffffu - (uint32_t)p); }
+__device__ __forceinline__ float val_of(uint64_t p) { return value_of((uint32_t)(p >> 32)); }
+
+struct RowOut {
+  const int64_t* target64;
+  const int32_t* target32;
+  int64_t ignore;
+  float* logp;
+  float* entropy;
+  float* top_logp;
+  int64_t* top_idx;
+  float4* stats;               // row maximum, log2 of the sum, entropy, - (NULL: no backward pass will follow)
+};
+
+struct Sums {
+  float m, s, a;               // maximum, sum of e, sum of e * y in units of log2
+};
+
+// what a row's sums say: (log of the sum, entropy) in nats; the row without a finite maximum has no probabilities
+struct RowStat {
+  float m, l2, h;
+  bool empty;
+};
+__device__ __forceinline__ RowStat stat_of(Sums q) {
+  RowStat r;
+  r.m = q.m;
+  r.empty = q.s == 0.f;                          // every entry is -inf
+  r.l2 = r.empty ? __builtin_inff() : log2f(q.s);
+  r.h = r.empty ? 0.f : (r.l2 - q.a / q.s) * kLn2;
+  return r;
+}
+__device__ __forceinline__ float logp_of(float x, RowStat r, float inv_t) {
+  if (r.empty) return -__builtin_inff();
+  return (x - r.m) * inv_t - r.l2 * kLn2;
+}
+
+template <class T>
+__device__ __forceinline__ void write_row(const T* __restrict__ x, int64_t cols, int64_t row, RowStat r, float inv_t,
+                                          const RowOut& o) {
+  const int64_t t = o.target64 ? o.target64[row] : (int64_t)o.target32[row];
+  float lp;
+  if (t == o.ignore) lp = 0.f;
+  else if (t < 0 || t >= cols) lp = __builtin_nanf("");
+  else lp = logp_of((float)x[t], r, inv_t);
+  o.logp[row] = lp;
+  o.entropy[row] = r.h;
+  if (o.stats) o.stats[row] = make_float4(r.m, r.l2, r.h, 0.f);
+}
+
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+  Sums r;
+  r.m = fmaxf(a.m, b.m);
+  r.s = 0.f;
+  r.a = 0.f;
+  if (a.s != 0.f) {                              // NaN counts
+    const float d = (a.m - r.m) * c, f = exp2f(d);
+    r.s += a.s * f;
+    r.a += f == 0.f ? 0.f : (a.a + d * a.s) * f;
+  }
+  if (b.s != 0.f) {
+    const float d = (b.m - r.m) * c, f = exp2f(d);
+    r.s += b.s * f;
+    r.a += f == 0.f ? 0.f : (b.a + d * b.s) * f;
+  }
+  return r;
+}
+
+// the k best of n pairs in LDS, in order, to out[0, k): a pair's place is the number of better ones
+template <class PUT>
+__device__ __forceinline__ void rank_pairs(const uint64_t* __restrict__ pairs, int n, int k, PUT put) {
+  for (int j = threadIdx.x; j < n; j += kBlock) {
+    const uint64_t mine = pairs[j];
+    int r = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) r += pairs[i] > mine;
+    if (r < k) put(r, mine);
+  }
+}
+
+// Exactly the k best of the `mine` columns from x on, in no order: for slices in which the bound leaves more candidates than
+// are ranked (many equal values, few finite ones). The k-th largest value by its bits, then, among the entries equal to it,
+// the last column that is still taken; the columns are read again from the caches for each count.
+template <class T>
+__device__ __attribute__((noinline)) void pick_exactly(const T* __restrict__ x, int mine, int k, int64_t c0, uint64_t* pairs,
+                                                       int* n_pairs, int* count) {
+  int turn = 0;
+  auto total = [&](int h) {                                     // over the block; the same for every thread
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) h += __shfl_xor(h, m, 64);
+    if ((threadIdx.x & 63) == 0) count[turn * kWaves + (threadIdx.x >> 6)] = h;
+    __syncthreads();
+    const int* q = count + turn * kWaves;
+    turn ^= 1;
+    return (q[0] + q[1]) + (q[2] + q[3]);
+  };
+  uint32_t kth = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cnd = kth | (1u << bit);
+    int h = 0;
+    for (int at = threadIdx.x; at < mine; at += kBlock) h += order_of((float)x[at]) >= cnd;
+    if (total(h) >= k) kth = cnd;
+  }
+  int above = 0;
+  for (int at = threadIdx.x; at < mine; at += kBlock) above += order_of((float)x[at]) > kth;
+  const int need = k - total(above);
+  int last = 0;                                                 // the need-th of the equal ones stands at this column
+  for (int bit = 16; bit >= 0; --bit) {
+    const int cnd = last | (1 << bit);
+    int h = 0;
+    for (int at = threadIdx.x; at < min(mine, cnd); at += kBlock) h += order_of((float)x[at]) == kth;
+    if (total(h) < need) last = cnd;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *n_pairs = 0;
+  __syncthreads();
+  for (int at = threadIdx.x; at < mine; at += kBlock) {
+    const float f = (float)x[at];
+    const uint32_t key = order_of(f);
+    if (key > kth || (key == kth && at <= last)) pairs[atomicAdd(n_pairs, 1)] = pair_of(f, c0 + at);
+  }
+}
+
+// ---- forward: slices --------------------------------------------------------------------------------------------------
+// Block (row, slice): columns [slice * len, ...). NV vectors a thread; vector v of thread t starts at column
+// (v * kBlock + t) * N of the slice. sums [rows][splits], cand [rows][splits][k]. With one slice a row the block writes the
+// row's results itself.
+template <class T, int NV, bool FULL, bool TOP>
+__global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ X, int64_t ldx, int64_t cols, int len,
+                                                          int splits, float c, float inv_t, int k, RowOut o,
+                                                          Sums* __restrict__ sums, uint64_t* __restrict__ cand) {
+  constexpr int N = Vec<T>::N;
+  typedef typename Vec<T>::raw R;
+  __shared__ float red[3 * kWaves];
+  __shared__ uint32_t bound[kWaves];
+  __shared__ uint64_t pairs[TOP ? kCand : 1];
+  __shared__ int n_pairs;
+  __shared__ int count[2 * kWaves];
+  const int64_t row = blockIdx.x / splits;
+  const int slice = (int)(blockIdx.x % splits);
+  const int64_t c0 = (int64_t)slice * len;
+  const int mine = (int)min((int64_t)len, cols - c0);           // columns of this slice
+  const T* x = X + row * ldx;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+
+  R raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int at = (v * kBlock + threadIdx.x) * N;
+    raw[v] = (R)(T)(-__builtin_inff());
+    if (FULL) {
+      if (at < mine) raw[v] = load_raw<T, true>(x + c0 + at, N);
+    } else if (at + N <= mine) {
+      raw[v] = load_raw<T, true>(x + c0 + at, N);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (at + e < mine) raw[v][e] = x[c0 + at + e];
+    }
+  }
+  float tm = -__builtin_inff();
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < N; ++e) tm = fmaxf(tm, (float)raw[v][e]);
+  float m = group_max<64>(tm);
+  if (lane == 0) red[w] = m;
+  if (threadIdx.x == 0) n_pairs = 0;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float base = m == -__builtin_inff() ? 0.f : m;          // nothing but -inf (and NaN): y = -inf, e = 0
+  float s = 0.f, a = 0.f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float y = ((float)raw[v][e] - base) * c;
+      const float p = __builtin_amdgcn_exp2f(y);
+      s += p;
+      a = fmaf(p, fmaxf(y, kFar), a);                           // a NaN is in p as well
+    }
+  const bool odd = s != s;                                      // this thread holds a NaN (or the row an infinity)
+  s = group_sum<64>(s);
+  a = group_sum<64>(a);
+  if (lane == 0) {
+    red[kWaves + w] = s;
+    red[2 * kWaves + w] = a;
+  }
+  if (TOP) {
+    // lower bound of the k-th largest value: as many threads as alternatives have a maximum that is no smaller. Each full
+    // wave of threads with columns finds the q-th largest of its threads' maxima, the smallest of these is the bound.
+    const int held = min(kBlock, (mine + N - 1) / N), full = max(1, held / 64), q = (k + full - 1) / full;
+    uint32_t t = w < full ? 0u : 0xffffffffu;
+    if (w < full && q <= 64) {
+      const uint32_t key = order_of(tm);
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cnd = t | (1u << bit);
+        const int n = __popcll(__ballot(key >= cnd));
+        if (n >= q) t = cnd;
+        if (n == q) break;
+      }
+    }
+    if (lane == 0) bound[w] = t;
+  }
+  __syncthreads();
+  Sums z;
+  z.m = m;
+  z.s = (red[kWaves] + red[kWaves + 1]) + (red[kWaves + 2] + red[kWaves + 3]);
+  z.a = (red[2 * kWaves] + red[2 * kWaves + 1]) + (red[2 * kWaves + 2] + red[2 * kWaves + 3]);
+  const RowStat r = stat_of(z);
+  if (threadIdx.x == 0) {
+    if (splits == 1) write_row(x, cols, row, r, inv_t, o);
+    else sums[blockIdx.x] = z;
+  }
+  if (!TOP) return;
+
+  const uint32_t tb = min(min(bound[0], bound[1]), min(bound[2], bound[3]));
+  // tb = 0: no bound. NaN is above every bound: !(x < tf)
+  const float tf = tb == 0 ? -__builtin_inff() : value_of(tb);
+  if (!(tm < tf) || odd) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float f = (float)raw[v][e];
+        const int at = (v * kBlock + threadIdx.x) * N + e;
+        if (!(f < tf) && at < mine) {
+          const int i = atomicAdd(&n_pairs, 1);
+          if (i < kCand) pairs[i] = pair_of(f, c0 + at);
+        }
+      }
+  }
+  __syncthreads();
+  int n = n_pairs;
+  if (n > kCand) {
+    pick_exactly<T>(x + c0, mine, k, c0, pairs, &n_pairs, count);
+    __syncthreads();
+    n = n_pairs;
+  }
+  if (splits == 1) {
+    rank_pairs(pairs, n, k, [&](int i, uint64_t p) {
+      o.top_idx[row * k + i] = col_of(p);
+      o.top_logp[row * k + i] = logp_of(val_of(p), r, inv_t);
+    });
+  } else {
+    uint64_t* out = cand + (int64_t)blockIdx.x * k;
+    rank_pairs(pairs, n, k, [&](int i, uint64_t p) { out[i] = p; });
+    for (int i = n + threadIdx.x; i < k; i += kBlock) out[i] = 0;
+  }
+}
+
+// ---- forward: the slices of a row -------------------------------------------------------------------------------------
+// sums of a row, by one wave; every lane ends with them. The order is fixed by the lane and the shuffles.
+__device__ __forceinline__ Sums row_sums(const Sums* __restrict__ p, int splits, float c) {
+  const int lane = threadIdx.x & 63;
+  Sums z = {-__builtin_inff(), 0.f, 0.f};
+  for (int i = lane; i < splits; i += 64) z = join(z, p[i], c);
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    Sums y;
+    y.m = __shfl_xor(z.m, m, 64);
+    y.s = __shfl_xor(z.s, m, 64);
+    y.a = __shfl_xor(z.a, m, 64);
+    z = (lane & m) ? join(y, z, c) : join(z, y, c);             // the same operands in the same order on both lanes
+  }
+  return z;
+}
+
+template <class T>
+__global__ __launch_bounds__(kBlock) void lp_join_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows, int64_t cols,
+                                                         int splits, float c, float inv_t, RowOut o,
+                                                         const Sums* __restrict__ sums) {
+  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));
+  if ((threadIdx.x & 63) == 0) write_row(X + row * ldx, cols, row, r, inv_t, o);
+}
+
+// ... with alternatives: one block a row. The slices' k best are pairs of distinct numbers: the k-th largest is found by its
+// bits (64 counts at most), the k that are left are ranked.
+template <class T>
+__global__ __launch_bounds__(kBlock) void lp_join_top_kernel(const T* __restrict__ X, int64_t ldx, int64_t cols, int splits,
+                                                             float c, float inv_t, int k, RowOut o,
+                                                             const Sums* __restrict__ sums,
+                                                             const uint64_t* __restrict__ cand) {
+  constexpr int kHold = 4096, kDirect = 256;
+  __shared__ uint64_t held[kHold];
+  __shared__ uint64_t best[kDirect];
+  __shared__ int n_best;
+  const int64_t row = blockIdx.x;
+  const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));
+  if (threadIdx.x == 0) {
+    write_row(X + row * ldx, cols, row, r, inv_t, o);
+    n_best = 0;
+  }
+  const int64_t total = (int64_t)splits * k;
+  const uint64_t* src = cand + row * total;
+  auto put = [&](int i, uint64_t p) {
+    o.top_idx[row * k + i] = col_of(p);
+    o.top_logp[row * k + i] = logp_of(val_of(p), r, inv_t);
+  };
+  if (total <= kDirect) {
+    uint64_t p = 0;
+    if ((int)threadIdx.x < total) p = src[threadIdx.x];
+    __syncthreads();
+    if (p) best[atomicAdd(&n_best, 1)] = p;
+    __syncthreads();
+    rank_pairs(best, n_best, k, put);
+    return;
+  }
+  const bool hold = total <= kHold;
+  if (hold)
+    for (int64_t i = threadIdx.x; i < total; i += kBlock) held[i] = src[i];
+  __syncthreads();
+  uint64_t t = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t cnd = t | (1ull << bit);
+    int h = 0;
+    if (hold)
+      for (int64_t i = threadIdx.x; i < total; i += kBlock) h += held[i] >= cnd;
+    else
+      for (int64_t i = threadIdx.x; i < total; i += kBlock) h += src[i] >= cnd;
+    // counts of a thread are small: the block's count is exact in fp32 too, but stays whole here
+    __shared__ int wsum[2][kWaves];
+    int ws = h;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) ws += __shfl_xor(ws, m, 64);
+    if ((threadIdx.x & 63) == 0) wsum[bit & 1][threadIdx.x >> 6] = ws;
+    __syncthreads();
+    const int n = (wsum[bit & 1][0] + wsum[bit & 1][1]) + (wsum[bit & 1][2] + wsum[bit & 1][3]);
+    if (n >= k) t = cnd;
+    if (n == k) break;
+  }
+  for (int64_t i = threadIdx.x; i < total; i += kBlock) {
+    const uint64_t p = src[i];
+    if (p && p >= t) {
+      const int j = atomicAdd(&n_best, 1);
+      if (j < kDirect) best[j] = p;
+    }
+  }
+  __syncthreads();
+  rank_pairs(best, min(n_best, kDirect), k, put);
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------
+template <class T, int NV, bool FULL>
+__global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X, int64_t ldx, int64_t cols, int splits,
+                                                        float c, float inv_t, int k, const int64_t* __restrict__ target64,
+                                                        const int32_t* __restrict__ target32, int64_t ignore,
+                                                        const int64_t* __restrict__ top_idx,
+                                                        const float4* __restrict__ stats, const float* __restrict__ glogp,
+                                                        const float* __restrict__ gent, const float* __restrict__ gtop,
+                                                        T* __restrict__ GX) {
+  constexpr int N = Vec<T>::N, LEN = kBlock * NV * N;
+  typedef typename Vec<T>::f32 F;
+  const int64_t row = blockIdx.x / splits;
+  const int64_t c0 = (int64_t)(blockIdx.x % splits) * LEN;
+  const T* x = X + row * ldx;
+  T* gx = GX + row * cols;
+  typename Vec<T>::raw raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t at = c0 + (v * kBlock + threadIdx.x) * N;
+    if (at < cols) raw[v] = load_raw<T, FULL>(x + at, (int)min((int64_t)N, cols - at));
+  }
+  const float4 st = stats[row];
+  const bool empty = st.y == __builtin_inff();
+  const float m = empty ? 0.f : st.x, l2 = empty ? 0.f : st.y;
+  const int64_t t = target64 ? target64[row] : (int64_t)target32[row];
+  const float gt = (glogp && t != ignore) ? glogp[row] : 0.f;
+  float g = gt;
+  if (gtop)
+    for (int i = 0; i < k; ++i) g += gtop[row * k + i];
+  const float gh = gent ? gent[row] : 0.f;
+  // gx = p (a + b log2 p) away from the named columns
+  const float a = -inv_t * (g + gh * st.z), b = -inv_t * gh * kLn2;
+  auto common = [&](float f) {
+    const float q = fmaf(f - m, c, -l2);
+    const float p = __builtin_amdgcn_exp2f(q);
+    return p * fmaf(b, fmaxf(q, kFar), a);
+  };
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t at = c0 + (v * kBlock + threadIdx.x) * N;
+    if (at < cols) {
+      const F f = to_f32<T>(raw[v]);
+      F y;
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[e] = empty ? 0.f : common(f[e]);
+      store_f32<T, FULL>(gx + at, (int)min((int64_t)N, cols - at), y);
+    }
+  }
+  // the named columns of this slice once more, with their own part: entry 0 is the target, the others the alternatives. One
+  // thread a column: the first entry that names it adds up all that do.
+  __threadfence_block();
+  __syncthreads();
+  const int named = 1 + (gtop ? k : 0);
+  for (int i = threadIdx.x; i < named; i += kBlock) {
+    const int64_t j = i ? top_idx[row * k + i - 1] : t;
+    if (j < c0 || j >= min(cols, c0 + LEN) || empty || (i == 0 && t == ignore)) continue;
+    if (i && j == t && t != ignore) continue;
+    float own = i ? gtop[row * k + i - 1] : gt;
+    if (i == 0 && gtop)
+      for (int h = 0; h < k; ++h)
+        if (top_idx[row * k + h] == j) own += gtop[row * k + h];
+    gx[j] = (T)(inv_t * own + common((float)x[j]));
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------
+struct Cut {
+  int nv;          // vectors a thread
+  int len;         // columns of a slice
+  int64_t splits;
+};
+
+// Slices as long as a block's registers hold (64 values a thread); shorter ones where that leaves fewer than 512 blocks.
+// Slices of a row are of equal length, to whole vectors.
+Cut cut_for(int64_t rows, int64_t cols, int es) {
+  const int n = 16 / es, most = 64 / n;
+  Cut q{};
+  for (q.nv = most; q.nv > 2; q.nv /= 2)
+    if (rows * ((cols + kBlock * n * q.nv - 1) / (kBlock * n * q.nv)) >= 512) break;
+  while (q.nv > 2 && (int64_t)kBlock * n * (q.nv / 2) >= cols) q.nv /= 2;
+  const int64_t most_len = (int64_t)kBlock * n * q.nv;
+  q.splits = (cols + most_len - 1) / most_len;
+  q.len = (int)(((cols + q.splits - 1) / q.splits + n - 1) / n * n);
+  q.splits = (cols + q.len - 1) / q.len;
+  return q;
+}
+
+size_t ws_bytes(int64_t rows, const Cut& q, int k) {
+  if (q.splits == 1) return 16;
+  const size_t sums = ((size_t)rows * q.splits * sizeof(Sums) + 15) / 16 * 16;
+  return sums + (size_t)rows * q.splits * k * 8 + 16;
+}
+
+int check_common(int dtype, int64_t rows, int64_t cols, int target_bytes, int k, float temperature) {
+  if (!known_dtype(dtype) || rows < 0 || cols < 1 || (target_bytes != 4 && target_bytes != 8) || k < 0) return MMSSL_E_BADARG;
+  if (!(temperature > 0.f) || temperature > 3.0e38f || !(1.0f / temperature <= 3.0e38f)) return MMSSL_E_BADARG;
+  if (k > kTopMax || k > cols || cols > 0x7ffffff0) return MMSSL_E_UNSUPP;
+  if (rows * ((cols + 2047) / 2048) > 0x3fffffff) return MMSSL_E_UNSUPP;     // blocks of a launch
+  return 0;
+}
+
+}  // namespace
+
+extern "C" size_t mmssl_logprobs_rows_workspace_bytes(int dtype, int64_t rows, int64_t cols, int k) {
+  if (check_common(dtype, rows, cols, 8, k, 1.0f)) return 0;
+  return ws_bytes(rows, cut_for(rows, cols, dtype_bytes(dtype)), k);
+}
+
+extern "C" int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_t rows, int64_t cols, const void* target,
+                                   int target_bytes, int64_t ignore_index, int k, float temperature, float* logp,
+                                   float* entropy, float* top_logp, int64_t* top_idx, float* stats, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  if (int rc = check_common(dtype, rows, cols, target_bytes, k, temperature)) return rc;
+  if (rows == 0) return 0;
+  const size_t es = dtype_bytes(dtype);
+  if (!X || !target || !logp || !entropy || ldx < 0 || (k > 0 && (!top_logp || !top_idx))) return MMSSL_E_BADARG;
+  if (!aligned_to(X, es) || !aligned_to(target, target_bytes) || !aligned_to(stats, 16) || !aligned_to(top_idx, 8))
+    return MMSSL_E_BADARG;
+  const Cut q = cut_for(rows, cols, (int)es);
+  if (q.splits > 1 && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < ws_bytes(rows, q, k)))
+    return MMSSL_E_WORKSPACE;
+  const float c = (float)((double)kLog2e / temperature), inv_t = (float)(1.0 / (double)temperature);
+  Sums* sums = static_cast<Sums*>(workspace);
+  uint64_t* cand = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) +
+                                               ((size_t)rows * q.splits * sizeof(Sums) + 15) / 16 * 16);
+  RowOut o{target_bytes == 8 ? static_cast<const int64_t*>(target) : nullptr,
+           target_bytes == 4 ? static_cast<const int32_t*>(target) : nullptr,
+           ignore_index, logp, entropy, top_logp, top_idx, reinterpret_cast<float4*>(stats)};
+  const hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)(rows * q.splits)), block(kBlock);
+#define LP_SLICE_T(T, V, F, TOP)                                                                                         \
+  hipLaunchKernelGGL((lp_slice_kernel<T, V, F, TOP>), grid, block, 0, s, (const T*)X, ldx, cols, q.len, (int)q.splits, c, \
+                     inv_t, k, o, sums, cand)
+#define LP_SLICE_V(T, V)                                         \
+  if constexpr (V * Vec<T>::N <= 64) {                           \
+    if (cols % Vec<T>::N == 0) {                                 \
+      if (k) LP_SLICE_T(T, V, true, true);                       \
+      else LP_SLICE_T(T, V, true, false);                        \
+    } else {                                                     \
+      if (k) LP_SLICE_T(T, V, false, true);                      \
+      else LP_SLICE_T(T, V, false, false);                       \
+    }                                                            \
+  }
+#define LP_SLICE(T)                      \
+  switch (q.nv) {                        \
+    case 16: LP_SLICE_V(T, 16); break;   \
+    case 8: LP_SLICE_V(T, 8); break;     \
+    case 4: LP_SLICE_V(T, 4); break;     \
+    default: LP_SLICE_V(T, 2); break;    \
+  }
+  MMSSL_BY_DTYPE(dtype, LP_SLICE);
+  MMSSL_LAUNCH_CHECK();
+  if (q.splits == 1) return 0;
+#define LP_JOIN(T)                                                                                                       \
+  if (k)                                                                                                                 \
+    hipLaunchKernelGGL(lp_join_top_kernel<T>, dim3((unsigned)rows), block, 0, s, (const T*)X, ldx, cols, (int)q.splits, c, \
+                       inv_t, k, o, (const Sums*)sums, (const uint64_t*)cand);                                           \
+  else                                                                                                                   \
+    hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), block, 0, s, (const T*)X, ldx,  \
+                       rows, cols, (int)q.splits, c, inv_t, o, (const Sums*)sums)
+  MMSSL_BY_DTYPE(dtype, LP_JOIN);
+  MMSSL_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int mmssl_logprobs_rows_bwd(const void* X, int64_t ldx, int dtype, int64_t rows, int64_t cols,
+                                       const void* target, int target_bytes, int64_t ignore_index, int k,
+                                       float temperature, const int64_t* top_idx, const float* stats, const float* glogp,
+                                       const float* gentropy, const float* gtop, void* GX, void* stream) {
+  if (int rc = check_common(dtype, rows, cols, target_bytes, k, temperature)) return rc;
+  if (rows == 0) return 0;
+  const size_t es = dtype_bytes(dtype);
+  if (!X || !target || !stats || !GX || ldx < 0 || (gtop && (!top_idx || k < 1))) return MMSSL_E_BADARG;
+  if (!aligned_to(X, es) || !aligned_to(GX, es) || !aligned_to(target, target_bytes) || !aligned_to(stats, 16) ||
+      !aligned_to(top_idx, 8))
+    return MMSSL_E_BADARG;
+  const float c = (float)((double)kLog2e / temperature), inv_t = (float)(1.0 / (double)temperature);
+  const int64_t* t64 = target_bytes == 8 ? static_cast<const int64_t*>(target) : nullptr;
+  const int32_t* t32 = target_bytes == 4 ? static_cast<const int32_t*>(target) : nullptr;
+  constexpr int NV = 4;
+#define LP_BWD_F(T, F)                                                                                                   \
+  hipLaunchKernelGGL((lp_bwd_kernel<T, NV, F>), dim3((unsigned)(rows * splits)), dim3(kBlock), 0, as_stream(stream),      \
+                     (const T*)X, ldx, cols, (int)splits, c, inv_t, k, t64, t32, ignore_index, top_idx,                  \
+                     (const float4*)stats, glogp, gentropy, gtop, (T*)GX)
+#define LP_BWD(T)                                                                         \
+  const int64_t splits = (cols + kBlock * NV * Vec<T>::N - 1) / (kBlock * NV * Vec<T>::N); \
+  if (cols % Vec<T>::N == 0) LP_BWD_F(T, true);                                           \
+  else LP_BWD_F(T, false)
+  MMSSL_BY_DTYPE(dtype, LP_BWD);
+  MMSSL_LAUNCH_CHECK();
+  return 0;
+}

@@ -1574,3 +1574,76 @@ def layernorm_rows(X, weight=None, bias=None, eps=1e-5):
                                     or (b is not None and b.requires_grad)):
         return _LayerNormRows.apply(X, w, b, float(eps))
     return _layernorm_fwd(X, w, b, float(eps), False)[0]
+
+
+LOGPROBS_MAX_K = 128
+
+
+def _logprobs_fwd(X, target, k, temperature, ignore_index, want_stats):
+    X2, ldx = _rows2d(X)
+    rows, cols = X2.shape
+    lead, dev = X.shape[:-1], X.device
+    out = torch.empty((2,) + lead, dtype=torch.float32, device=dev)
+    logp, entropy = out[0], out[1]
+    top_logp = torch.empty(lead + (k,), dtype=torch.float32, device=dev) if k else None
+    top_idx = torch.empty(lead + (k,), dtype=torch.int64, device=dev) if k else None
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
+    dt = _DTYPES[X.dtype]
+    nb = _lib.lib().mmssl_logprobs_rows_workspace_bytes(dt, rows, cols, k)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    _call("mmssl_logprobs_rows", X, X2.data_ptr(), ldx, dt, rows, cols, target.data_ptr(), target.element_size(), ignore_index,
+          k, temperature, logp.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_idx), _ptr(stats), ws.data_ptr(), nb)
+    return logp, entropy, top_logp, top_idx, X2, stats
+
+
+class _LogprobsRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, X, target, k, temperature, ignore_index):
+        logp, entropy, top_logp, top_idx, X2, stats = _logprobs_fwd(X, target, k, temperature, ignore_index, True)
+        ctx.save_for_backward(X2 if X.dim() != 2 else X, target, stats, top_idx)
+        ctx.cfg = (X.shape, k, temperature, ignore_index)
+        ctx.set_materialize_grads(False)
+        if top_idx is not None:
+            ctx.mark_non_differentiable(top_idx)
+        return logp, entropy, top_logp, top_idx
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        X, target, stats, top_idx = ctx.saved_tensors
+        shape, k, temperature, ignore_index = ctx.cfg
+        if g_logp is None and g_entropy is None and g_top is None:
+            return None, None, None, None, None
+        X2, ldx = _rows2d(X)
+        rows, cols = X2.shape
+        g_logp, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top))
+        gx = torch.empty(shape, dtype=X2.dtype, device=X2.device)
+        _call("mmssl_logprobs_rows_bwd", X2, X2.data_ptr(), ldx, _DTYPES[X2.dtype], rows, cols, target.data_ptr(),
+              target.element_size(), ignore_index, k, temperature, _ptr(top_idx), stats.data_ptr(), _ptr(g_logp),
+              _ptr(g_entropy), _ptr(g_top), gx.data_ptr())
+        return gx, None, None, None, None
+
+
+def logprobs_rows(X, target, k=0, temperature=1.0, ignore_index=-100):
+    """What score rows X [..., n] (fp32 / bf16 / fp16) say at `temperature` as distributions over their n columns:
+    (logp, entropy, top_logp, top_idx) = the log probability of column target[...] (int64 or int32), the entropy in nats, and
+    the k best columns' log probabilities and numbers [..., k] (descending, ties by ascending column like topk_rows; k <= 128;
+    None for k = 0). fp32 results with fp32 sums; X is read once, n * rows probabilities are never stored.
+    Masked columns hold -inf: probability 0. A row of nothing else has logp -inf, entropy 0, gradient 0. `ignore_index` as a
+    target: logp 0 and no gradient from it; any other target outside the row: logp NaN. A NaN or +inf in a row makes its logp
+    and entropy NaN. Differentiable in X through logp, entropy and top_logp."""
+    _typed(X, "X")
+    k = int(k)
+    if X.dim() < 1 or X.shape[-1] < 1:
+        raise _lib.MmsslError("logprobs_rows: X must be [..., n] with n >= 1")
+    if k < 0 or k > LOGPROBS_MAX_K or k > X.shape[-1]:
+        raise _lib.MmsslError("logprobs_rows: 0 <= k <= min(%d, n) expected, got %d" % (LOGPROBS_MAX_K, k))
+    temperature = float(temperature)
+    if not 1e-30 <= temperature <= 1e30:
+        raise _lib.MmsslError("logprobs_rows: temperature must be a positive number, got %r" % (temperature,))
+    target = _tokens(target, "target", X.device)
+    if target.shape != X.shape[:-1]:
+        raise _lib.MmsslError("logprobs_rows: target must be %s, got %s" % (list(X.shape[:-1]), list(target.shape)))
+    if X.requires_grad and torch.is_grad_enabled():
+        return _LogprobsRows.apply(X, target, k, temperature, int(ignore_index))
+    return _logprobs_fwd(X, target, k, temperature, int(ignore_index), False)[:4]

@@ -306,3 +306,253 @@ def test_layernorm_gradient_against_differences():
         mine = float((grads[k].cpu().double() * u).sum())
         # differences: e^2 of the third derivative and 1e-16 / e of rounding, both far below the 32-bit sums' share
         assert abs(mine - slope) <= 1e-5 * float((grads[k].cpu().double().abs() * u.abs()).sum()) + 1e-6, (k, mine, slope)
+
+
+# ---- logprobs_rows ----------------------------------------------------------------------------------------------------
+def logprobs_exact(x, target, k, temperature, ignore, grads=None):
+    """(logp, entropy, top_logp, top_idx[, gx]) in 64 bits."""
+    z = x.double() / temperature
+    n, cols = z.shape
+    empty = torch.isneginf(z).all(1)
+    top = z.amax(1, keepdim=True)
+    u = z - torch.where(empty[:, None], torch.zeros_like(top), top)       # off first: a row of the type's lowest value is even
+    lp = u - torch.log(torch.exp(u).sum(1, keepdim=True))
+    lp[empty] = float("-inf")
+    p = lp.exp()
+    held = torch.where(p > 0, lp, torch.zeros_like(lp))            # 0 log 0 = 0
+    h = -(p * held).sum(1)
+    row = torch.arange(n)
+    ok = (target >= 0) & (target < cols)
+    logp = torch.where(ok, lp[row, target.clamp(0, cols - 1).long()], torch.full((n,), float("nan"), dtype=torch.float64))
+    logp[target == ignore] = 0.0
+    # descending value, ties by ascending column; torch sorts NaN above +inf
+    idx = torch.sort(x.double(), dim=1, descending=True, stable=True).indices[:, :k]
+    held32 = lambda v: torch.where(v < torch.finfo(torch.float32).min, float("-inf"), v)      # noqa: E731  (fp32 outputs)
+    outs = [held32(logp), h, held32(lp.gather(1, idx)), idx]
+    if grads is not None:
+        gl, gh, gt = (g.double() for g in grads)
+        gl = torch.where(target == ignore, torch.zeros_like(gl), gl)
+        named = torch.zeros_like(z)
+        named[row[ok & (target != ignore)], target[ok & (target != ignore)].long()] += gl[ok & (target != ignore)]
+        named.scatter_add_(1, idx, gt)
+        gx = named - p * (gl + gt.sum(1))[:, None] - gh[:, None] * p * (held + h[:, None])
+        gx[empty] = 0.0
+        outs.append(gx / temperature)
+    return outs
+
+
+def check_logprobs(x, k=0, temperature=1.0, target=None, ignore=-100, grad=True, seed=0):
+    from mmssl_amd import ops
+    n, cols = x.shape
+    g0 = gen(seed + 77)
+    if target is None:
+        target = torch.randint(cols, (n,), generator=g0)
+    grads = [torch.randn(n, generator=g0), torch.randn(n, generator=g0), torch.randn(n, k, generator=g0)]
+    want = logprobs_exact(x, target, k, temperature, ignore, grads)
+    xd = x.to(DEV).requires_grad_(True)
+    got = ops.logprobs_rows(xd, target.to(DEV), k=k, temperature=temperature, ignore_index=ignore)
+    # exp2 of y log2 e / T: two roundings of y and one unit of the instruction let a term be off by 2^-23 (1 + |y|) of itself,
+    # and |y| e^y <= 1; a sum of `cols` terms by 2^-24 of itself for each level of its tree and each of a thread's 64 adds
+    # in a row, the joins of slices more
+    rel = (64 + 20 + cols / 16384) * 2.0 ** -24 + 3 * 2.0 ** -23
+    # (x - m) / T - log S: |x - m| / T <= |logp|, three roundings of it
+    within(got[0], want[0], want[0].abs().nan_to_num(posinf=0.0) * 2.0 ** -22 + rel, "logp")
+    eh = rel * (2 + 2 * want[1].abs().nan_to_num())
+    within(got[1], want[1], eh, "entropy")
+    if k:
+        assert torch.equal(got[3].cpu(), want[3]), ("top_idx", (got[3].cpu() != want[3]).nonzero()[:3])
+        within(got[2], want[2], want[2].abs().nan_to_num(posinf=0.0) * 2.0 ** -22 + rel, "top_logp")
+    else:
+        assert got[2] is None and got[3] is None
+    if grad:
+        outs, gs = list(got[:2]), grads[:2]
+        if k:
+            outs.append(got[2])
+            gs.append(grads[2])
+        (gx,) = torch.autograd.grad(outs, xd, [g.to(DEV) for g in gs])
+        t = x.dtype
+        gl, gh, gt = (g.double().abs() for g in grads)
+        # p is off by the sum's share and by |log p| roundings of the exponent; the entropy's factor by the same again
+        size = gl + gt.sum(1) + gh * (2 + want[1].abs().nan_to_num())
+        bound = want[4].abs() * half_step(t) * 2 + (size * (rel * 6 + 40 * 2.0 ** -23) / temperature)[:, None]
+        bound = bound + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+        within(gx, want[4], bound.nan_to_num(), "gx")
+    with torch.no_grad():
+        again = ops.logprobs_rows(xd, target.to(DEV), k=k, temperature=temperature, ignore_index=ignore)
+    for a, b in zip(got, again):
+        assert (a is None and b is None) or torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0))
+    return got
+
+
+def scores(n, cols, t, seed, masked=0.0, scale=3.0):
+    g0 = gen(seed)
+    x = torch.randn(n, cols, generator=g0) * scale
+    if masked:
+        x[torch.rand(n, cols, generator=g0) < masked] = float("-inf")
+    return x.to(t)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n,cols,k", [(1, 1, 1), (3, 2, 2), (2, 7, 5), (5, 64, 10), (4, 65, 64), (3, 255, 100), (2, 500, 128),
+                                      (7, 1000, 20), (3, 1025, 128), (2, 1500, 128), (5, 2048, 50), (2, 2500, 128),
+                                      (1, 4099, 1), (3, 16384, 20), (3, 16385, 50), (2, 40001, 128), (1, 100000, 20)])
+def test_logprobs_rows(n, cols, k, t):
+    check_logprobs(scores(n, cols, t, cols), k=k, seed=k)
+    check_logprobs(scores(n, cols, t, cols + 1, masked=0.3), k=0, seed=k)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_logprobs_many_rows_whole_slices_and_one_launch(t):
+    """From 512 blocks on the slices are as long as the registers hold; short rows are done in one launch."""
+    check_logprobs(scores(1100, 1300, t, 1), k=10)
+    check_logprobs(scores(530, 9000, t, 2, masked=0.1), k=50)
+    check_logprobs(scores(300, 33001, t, 3), k=0)
+    check_logprobs(scores(260, 17000, t, 4), k=3)
+
+
+@pytest.mark.parametrize("cols", [100, 900, 3000, 70000])
+def test_logprobs_rows_of_equal_and_masked_values(cols):
+    """Ties go to the lowest column, whatever their number; rows that the mask leaves little or nothing of; masks of the
+    type's lowest value."""
+    inf = float("inf")
+    for t in TYPES:
+        low = torch.finfo(t).min
+        x = torch.zeros(12, cols)
+        g0 = gen(cols)
+        x[1] = 2.0
+        x[1, cols // 2] = 3.0
+        x[2] = -inf
+        x[3] = -inf
+        x[3, cols - 1] = 1.0
+        x[4] = -inf
+        x[4, [5, cols // 3, cols - 2]] = torch.tensor([0.5, 0.5, 4.0])
+        x[5] = torch.randint(0, 3, (cols,), generator=g0).float()
+        x[6] = low
+        x[7] = low
+        x[7, 3] = 0.0
+        x[8] = torch.where(torch.rand(cols, generator=g0) < 0.99, -inf, 0.0)
+        x[9, ::2] = -0.0
+        x[10] = torch.randn(cols, generator=g0).round()
+        x[11] = -inf
+        x[11, :cols // 2] = low
+        x = x.to(t)
+        for k in (0, 1, 20, 100):
+            target = torch.randint(cols, (12,), generator=g0)
+            check_logprobs(x, k=k, target=target)
+            check_logprobs(x, k=k, target=target, temperature=0.7, grad=False)
+
+
+def test_logprobs_of_nan_and_infinite_scores():
+    from mmssl_amd import ops
+    for cols in (50, 5000):
+        x = torch.randn(6, cols, generator=gen(3))
+        x[0, 7] = float("nan")
+        x[1, 8] = float("inf")
+        x[2] = float("nan")
+        x[3] = float("-inf")
+        x[3, 4] = float("nan")
+        x[4, 9] = float("nan")
+        x[4, 3] = float("inf")
+        for t in TYPES:
+            v = x.to(t)
+            logp, h, tl, ti = ops.logprobs_rows(v.to(DEV), torch.zeros(6, dtype=torch.int32, device=DEV), k=5)
+            assert bool(logp[:5].isnan().all()) and bool(h[:5].isnan().all()) and bool(logp[5].isfinite())
+            want = torch.sort(v.double(), dim=1, descending=True, stable=True).indices[:, :5]
+            assert torch.equal(ti.cpu(), want)
+            assert bool(tl[:3].isnan().all())
+
+
+def test_logprobs_targets_that_name_no_column():
+    x = scores(9, 1234, torch.float32, 5)
+    target = torch.tensor([0, 1233, -100, 1234, -1, 1 << 40, 5, -(1 << 40), -100])
+    check_logprobs(x, k=4, target=target)
+    check_logprobs(x, k=4, target=target, ignore=-1)
+    check_logprobs(x, k=0, target=target[[0, 1, 2, 3, 4, 6, 6, 2, 2]].int())
+
+
+def test_logprobs_temperature_and_large_scores():
+    for temperature in (0.05, 0.5, 1.0, 3.0, 100.0):
+        for t in TYPES:
+            check_logprobs(scores(4, 3001, t, 9), k=7, temperature=temperature)
+    x = scores(4, 5000, torch.float32, 10) + 10000.0               # far from zero: the maximum is taken off first
+    check_logprobs(x, k=5)
+    check_logprobs(scores(3, 2000, torch.float32, 11, scale=200.0), k=5)
+    x = scores(3, 2000, torch.float32, 11)
+    x[0] = x[0] * 1e37
+    x[1, 5] = 3e38
+    x[1, 6] = -3e38
+    check_logprobs(x, k=5, grad=False)
+
+
+def test_logprobs_shapes_strides_and_empty_inputs():
+    from mmssl_amd import ops
+    wide = scores(24, 701, torch.float32, 12)
+    target = torch.randint(600, (24,), generator=gen(1))
+    for t in TYPES:
+        w = wide.to(t).to(DEV)
+        for x in (w[:, 7:650], w[:, :643], w[:1, :643].expand(24, 643), w[:, :643].t().contiguous().t()):
+            tg = target.to(DEV)
+            a = x.detach().requires_grad_(True)
+            b = x.detach().contiguous().requires_grad_(True)
+            oa, ob = ops.logprobs_rows(a, tg, k=6), ops.logprobs_rows(b, tg, k=6)
+            assert all(torch.equal(u, v) for u, v in zip(oa, ob))
+            ga = torch.autograd.grad(oa[0].sum() + oa[1].mean(), a)[0]
+            gb = torch.autograd.grad(ob[0].sum() + ob[1].mean(), b)[0]
+            assert torch.equal(ga, gb)
+        c = w[:, :640].reshape(2, 3, 4, 640)
+        o3 = ops.logprobs_rows(c, tg.reshape(2, 3, 4), k=3)
+        o2 = ops.logprobs_rows(c.reshape(24, 640), tg, k=3)
+        assert o3[0].shape == (2, 3, 4) and o3[3].shape == (2, 3, 4, 3)
+        assert all(torch.equal(u.reshape(v.shape), v) for u, v in zip(o3, o2))
+    one = ops.logprobs_rows(wide[0].to(DEV), torch.tensor(5, device=DEV), k=2)
+    assert one[0].shape == () and one[3].shape == (2,)
+    e = torch.zeros(0, 40, device=DEV, requires_grad=True)
+    o = ops.logprobs_rows(e, torch.zeros(0, dtype=torch.int64, device=DEV), k=3)
+    assert o[0].shape == (0,) and o[2].shape == (0, 3)
+    assert torch.autograd.grad(o[0].sum(), e)[0].shape == (0, 40)
+    # each output by itself, and the gradient of a sum where all of them meet
+    x = scores(5, 333, torch.float32, 13).to(DEV).requires_grad_(True)
+    tg = torch.arange(5, device=DEV)
+    o = ops.logprobs_rows(x, tg, k=4)
+    parts = [torch.autograd.grad(o[i].sum(), x, retain_graph=True)[0] for i in range(3)]
+    whole = torch.autograd.grad(o[0].sum() + o[1].sum() + o[2].sum(), x)[0]
+    assert float((sum(parts) - whole).abs().max()) <= 1e-5
+
+
+def test_logprobs_gradient_against_differences():
+    from mmssl_amd import ops
+    g0 = gen(21)
+    x = torch.randn(4, 50, generator=g0) * 2
+    target = torch.tensor([3, 49, 0, -100])
+    c = [torch.randn(4, generator=g0).double(), torch.randn(4, generator=g0).double(), torch.randn(4, 6, generator=g0).double()]
+
+    def f(v):
+        o = logprobs_exact(v, target, 6, 1.3, -100)
+        return float(sum((a * b).sum() for a, b in zip(o[:3], c)))
+
+    xd = x.to(DEV).requires_grad_(True)
+    o = ops.logprobs_rows(xd, target.to(DEV), k=6, temperature=1.3)
+    (gx,) = torch.autograd.grad(sum((a * b.float().to(DEV)).sum() for a, b in zip(o[:3], c)), xd)
+    for seed in range(4):
+        u = torch.randn(4, 50, generator=gen(seed)).double()
+        e = 1e-6
+        slope = (f(x.double() + e * u) - f(x.double() - e * u)) / (2 * e)
+        mine = float((gx.cpu().double() * u).sum())
+        assert abs(mine - slope) <= 2e-5 * float((gx.cpu().double().abs() * u.abs()).sum()) + 1e-5, (mine, slope)
+
+
+def test_logprobs_row_offsets_past_32_bits():
+    from mmssl_amd import ops
+    cols = 1 << 20
+    rows = 2100                                              # 2.2e9 columns of bf16: 4.4 GB
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x[-1, 77] = 3.0
+    x[-1, -1] = 2.0
+    x.requires_grad_(True)
+    target = torch.full((rows,), cols - 1, device=DEV)
+    o = ops.logprobs_rows(x, target, k=3)
+    assert o[3][-1].tolist() == [77, cols - 1, 0] and o[3][0].tolist() == [0, 1, 2]
+    lse = torch.logsumexp(x.detach()[-1].double(), 0)
+    assert abs(float(o[0][-1].double() - (2.0 - lse))) < 1e-5
+    (gx,) = torch.autograd.grad(o[0][-1], x)
+    assert not bool(gx[:-1].any()) and abs(float(gx[-1, -1]) - 1.0) < 2 ** -8 and float(gx[-1, 77]) < 0
