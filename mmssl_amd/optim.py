@@ -180,3 +180,103 @@ class FusedAdamW(torch.optim.Optimizer):
         for gi, val in steps.items():
             dev = self.param_groups[gi]["params"][0].device
             self._group_state(gi, dev)[0] = val
+
+
+# ---------------------------------------------------------------------------------------
+# global gradient norm and clipping (csrc/gradnorm.hip)
+# ---------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # MMSSL_F32 / BF16 / F16
+CLIP_EPS = 1e-6                                                         # torch.nn.utils.clip_grad_norm_'s
+
+
+def _grad_list(grads, what):
+    """The list's C arrays (pointers, sizes, type codes) after one look at every tensor."""
+    n = len(grads)
+    kinds = {(g.dtype, g.device) if isinstance(g, torch.Tensor) and g.layout == torch.strided else None for g in grads}
+    if None in kinds:
+        raise _lib.MmsslError("%s: dense tensors expected" % what)
+    if any(d not in _DTYPES for d, _ in kinds):
+        raise _lib.MmsslError("%s: gradients must be float32, bfloat16 or float16" % what)
+    devices = {d for _, d in kinds}
+    if len(devices) > 1 or any(d.type != "cuda" for d in devices):
+        raise _lib.MmsslError("%s: gradients must be on one CUDA (HIP) device: this package has no CPU path" % what)
+    if not all([g.is_contiguous() for g in grads]):
+        raise _lib.MmsslError("%s: gradients must be contiguous" % what)
+    ptrs = (_ct.c_void_p * n)(*[g.data_ptr() for g in grads])
+    numel = (_ct.c_int64 * n)(*[g.numel() for g in grads])
+    if len(kinds) == 1:
+        dtypes = (_ct.c_int32 * n)(*([_DTYPES[grads[0].dtype]] * n))
+    else:
+        dtypes = (_ct.c_int32 * n)(*[_DTYPES[g.dtype] for g in grads])
+    return ptrs, numel, dtypes
+
+
+def _norm_call(name, dev, args_of):
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        _lib.check(getattr(_lib.lib(), name)(*args_of(norm), _lib.stream_ptr()), name)
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(grads):
+    """The 2-norm of all elements of a list of gradients together (fp32 / bf16 / fp16, mixed, any sizes) as a 0-dim fp32 device
+    tensor: one launch per 96 tensors and a small one, 64-bit sums in a fixed order, nothing read back."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        raise _lib.MmsslError("grad_norm: no gradients")
+    ptrs, numel, dtypes = _grad_list(grads, "grad_norm")
+    dev = grads[0].device
+    nb = _lib.lib().mmssl_grad_norm_workspace_bytes(len(grads))
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    return _norm_call("mmssl_grad_norm", dev,
+                      lambda norm: (ptrs, numel, dtypes, len(grads), norm.data_ptr(), ws.data_ptr(), nb))
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, out=None):
+    """Scale a list of gradients down to the global norm `max_norm` (times min(1, max_norm / (norm + 1e-6))) and return the norm
+    they had, a 0-dim fp32 device tensor. `out`: where the scaled gradients go, one tensor of the same type and number of
+    elements per gradient (default: the gradients themselves; no two tensors may overlap otherwise). The factor never leaves
+    the device; a NaN among the gradients makes all of them NaN, an infinite norm the finite ones 0."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise _lib.MmsslError("clip_grads: max_norm must be a number >= 0, got %r" % (max_norm,))
+    if not grads:
+        raise _lib.MmsslError("clip_grads: no gradients")
+    ptrs, numel, dtypes = _grad_list(grads, "clip_grads")
+    dev = grads[0].device
+    if out is None:
+        optrs = ptrs
+    else:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(out) != len(grads):
+            raise _lib.MmsslError("clip_grads: %d outputs for %d gradients" % (len(out), len(grads)))
+        optrs, onumel, odtypes = _grad_list(out, "clip_grads: out")
+        if out[0].device != dev or bytes(onumel) != bytes(numel) or bytes(odtypes) != bytes(dtypes):
+            raise _lib.MmsslError("clip_grads: out must match the gradients' types, sizes and device")
+    written = [p for p, n in zip(optrs, numel) if n]
+    if len(set(written)) != len(written):
+        raise _lib.MmsslError("clip_grads: the same memory twice among the %s" % ("gradients" if out is None else "outputs"))
+    nb = _lib.lib().mmssl_grad_norm_workspace_bytes(len(grads))
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    return _norm_call("mmssl_clip_grads", dev,
+                      lambda norm: (ptrs, optrs, numel, dtypes, len(grads), max_norm, CLIP_EPS, norm.data_ptr(),
+                                    ws.data_ptr(), nb))
+
+
+def clip_grad_norm(parameters, max_norm):
+    """clip_grads over the `.grad` of the parameters that have one, in place (what a training loop calls between backward and
+    FusedAdamW.step). A gradient that is not contiguous is scaled through a contiguous copy."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        raise _lib.MmsslError("clip_grad_norm: no parameter has a gradient")
+    flat = [g if g.layout != torch.strided or g.is_contiguous() else g.contiguous() for g in grads]
+    norm = clip_grads(flat, max_norm)
+    with torch.no_grad():
+        for g, f in zip(grads, flat):
+            if f is not g:
+                g.copy_(f)
+    return norm

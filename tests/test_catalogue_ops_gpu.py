@@ -556,3 +556,228 @@ def test_logprobs_row_offsets_past_32_bits():
     assert abs(float(o[0][-1].double() - (2.0 - lse))) < 1e-5
     (gx,) = torch.autograd.grad(o[0][-1], x)
     assert not bool(gx[:-1].any()) and abs(float(gx[-1, -1]) - 1.0) < 2 ** -8 and float(gx[-1, 77]) < 0
+
+
+# ---- gradient norm and clipping ---------------------------------------------------------------------------------------
+def grad_lists():
+    g0 = gen(31)
+    sizes = [1, 2, 3, 8, 17, 255, 256, 8191, 8192, 8193, 100000, 0, 65536, 33333]
+    yield "one", [torch.randn(5, generator=g0)]
+    yield "fp32", [torch.randn(n, generator=g0) for n in sizes]
+    yield "mixed", [torch.randn(n, generator=g0).to(TYPES[i % 3]) for i, n in enumerate(sizes)]
+    yield "many", [(torch.randn(n % 700 + 1, generator=g0) * 0.01).to(TYPES[n % 2]) for n in range(300)]
+    yield "96", [torch.randn(40, generator=g0) for _ in range(96)]
+    yield "shapes", [torch.randn(30, 20, 7, generator=g0), torch.randn((), generator=g0), torch.randn(1000, 64, generator=g0)]
+    yield "large", [torch.randn(3000001, generator=g0).bfloat16(), torch.randn(9000000, generator=g0)]
+
+
+@pytest.mark.parametrize("name,grads", list(grad_lists()), ids=lambda v: v if isinstance(v, str) else "")
+def test_grad_norm_and_clipping(name, grads):
+    from mmssl_amd import optim
+    total = sum(float((g.double() ** 2).sum()) for g in grads) ** 0.5
+    dev = [g.to(DEV) for g in grads]
+    assert abs(float(optim.grad_norm(dev)) - total) <= total * (2.0 ** -24 + 1e-12)
+    for max_norm in (total * 0.3, total * 7, 0.0):
+        c = min(1.0, max_norm / (total + 1e-6))
+        out = [torch.full_like(g, 5.0) for g in dev]
+        n1 = optim.clip_grads(dev, max_norm, out=out)
+        mine = [g.clone() for g in dev]
+        n2 = optim.clip_grads(mine, max_norm)
+        params = [torch.nn.Parameter(torch.zeros_like(g)) for g in dev]
+        for p, g in zip(params, dev):
+            p.grad = g.clone()
+        n3 = optim.clip_grad_norm(params + [torch.nn.Parameter(torch.zeros(3, device=DEV))], max_norm)
+        for n in (n1, n2, n3):
+            assert n.shape == () and abs(float(n) - total) <= total * (2.0 ** -24 + 1e-12)
+        for g, a, b, p, d in zip(grads, out, mine, params, dev):
+            t = g.dtype
+            tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps
+            # the factor is rounded to 32 bits, so is the product, then the type
+            within(a, g.double() * c, (g.double() * c).abs() * (half_step(t) + 2.0 ** -22) + tiny, name)
+            assert torch.equal(a, b) and torch.equal(a, p.grad) and torch.equal(d.cpu(), g)
+            if c == 1.0:
+                assert torch.equal(a, d)
+
+
+def test_grad_norm_keeps_range_and_reports_what_is_not_finite():
+    from mmssl_amd import optim
+    for v in (1e-30, 1e30, 3e38):                            # squares that fp32 does not hold
+        g = [torch.full((1000,), v, device=DEV), torch.full((24,), v, device=DEV)]
+        want = 32.0 * float(torch.tensor(v)) if v < 1e37 else float("inf")
+        got = float(optim.grad_norm(g))
+        assert got == want or abs(got - want) <= want * 1e-7
+    g = [torch.full((10,), 3e38, device=DEV)]                # the norm passes fp32, the factor does not
+    optim.clip_grads(g, 1.0)
+    assert float((g[0] - 10 ** -0.5).abs().max()) < 1e-6
+    z = [torch.zeros(100, device=DEV)]
+    assert float(optim.clip_grads(z, 1.0)) == 0.0 and not bool(z[0].any())
+    a = [torch.ones(5, device=DEV), torch.tensor([1.0, float("inf")], device=DEV)]
+    assert float(optim.clip_grads(a, 1.0)) == float("inf")
+    assert not bool(a[0].any()) and bool(a[1][1].isnan())
+    b = [torch.ones(5, device=DEV), torch.tensor([1.0, float("nan")], device=DEV)]
+    n = optim.clip_grads(b, 1.0)
+    assert bool(n.isnan()) and bool(b[0].isnan().all())
+
+
+def test_clipping_unaligned_pieces_and_neighbours():
+    """Pieces of a flat buffer that begin anywhere: what lies between them is left as it was."""
+    from mmssl_amd import optim
+    g0 = gen(41)
+    for t in TYPES:
+        flat = torch.randn(60000, generator=g0).to(t)
+        cuts = [(1, 4), (7, 20), (33, 8192), (9001, 20000), (30003, 29997)]
+        dev = flat.to(DEV)
+        pieces = [dev[a:a + n] for a, n in cuts]
+        want = flat.double().clone()
+        total = sum(float((flat[a:a + n].double() ** 2).sum()) for a, n in cuts) ** 0.5
+        for a, n in cuts:
+            want[a:a + n] *= 0.5 * total / (total + 1e-6)
+        optim.clip_grads(pieces, 0.5 * total)
+        within(dev, want, want.abs() * (half_step(t) + 2.0 ** -22) + 1e-7, "flat")
+        keep = torch.ones(60000, dtype=torch.bool)
+        for a, n in cuts:
+            keep[a:a + n] = False
+        assert torch.equal(dev.cpu()[keep], flat[keep])
+    p = torch.nn.Parameter(torch.zeros(30, 50, device=DEV))
+    p.grad = torch.randn(50, 30, device=DEV).t()
+    was = p.grad.clone()
+    n = optim.clip_grad_norm([p], 1.0)
+    assert abs(float(n) - float(was.double().norm())) < 1e-4
+    assert float((p.grad - was / (n + 1e-6)).abs().max()) < 1e-6
+
+
+# ---- together ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_a_full_catalogue_model_trains_a_step(t):
+    """Histories -> rows -> norm -> scores against the item table -> log probabilities -> backward -> clipping -> AdamW, twice,
+    against the same in 64 bits on the host: losses, clipped gradients, weights."""
+    from mmssl_amd import ops, optim
+    g0 = gen(51)
+    items, d, b, length = 500, 64, 32, 20
+    table = (torch.randn(items, d, generator=g0) * 0.05).to(t)
+    w, bias = torch.ones(d).to(t), torch.zeros(d).to(t)
+    hist = torch.randint(-1, items, (b, length), generator=g0)            # -1: shorter histories
+    hist[3] = -1                                                          # one user without any
+    pos = torch.randint(items, (b,), generator=g0)
+    seen = torch.zeros(b, items, dtype=torch.bool)
+    seen.scatter_(1, hist.clamp(min=0), True)
+    seen[torch.arange(b), pos] = False
+    leaves = [torch.nn.Parameter(v.float().to(DEV)) for v in (table, w, bias)]      # fp32 master weights
+    opt = optim.FusedAdamW(leaves, lr=0.01, weight_decay=0.0)
+    ref = [v.double().clone().requires_grad_(True) for v in (table, w, bias)]
+    ropt = torch.optim.AdamW(ref, lr=0.01, weight_decay=0.0)
+    scale = d ** 0.5
+    tol = 2e-5 if t == torch.float32 else 4e-2
+    for step in range(2):
+        opt.zero_grad()
+        tab, ww, bb = (p.to(t) for p in leaves)
+        rows = ops.embed_rows(tab, hist.to(DEV), scale=scale, padding_idx=-1)
+        user = ops.layernorm_rows(rows.float().mean(1).to(t), ww, bb)
+        s = (user.float() @ tab.float().t()).masked_fill(seen.to(DEV), float("-inf"))
+        logp, entropy, _, top = ops.logprobs_rows(s, pos.to(DEV), k=5, temperature=0.5)
+        loss = -logp.mean() - 0.01 * entropy.mean()
+        loss.backward()
+        norm = optim.clip_grad_norm(leaves, 0.1)
+
+        ropt.zero_grad()
+        ok = (hist >= 0)[..., None]
+        rr = torch.where(ok, ref[0][hist.clamp(min=0)] * scale, torch.zeros((), dtype=torch.float64)).mean(1)
+        hu = (rr - rr.mean(1, keepdim=True)) / (rr.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt() * ref[1] + ref[2]
+        z = (hu @ ref[0].t()).masked_fill(seen, float("-inf")) / 0.5
+        lp = torch.log_softmax(z, 1)
+        h = -(lp.exp() * lp.masked_fill(seen, 0.0)).sum(1)
+        rloss = -lp[torch.arange(b), pos].mean() - 0.01 * h.mean()
+        rloss.backward()
+        rnorm = torch.nn.utils.clip_grad_norm_(ref, 0.1)
+        assert abs(float(loss.detach()) - float(rloss.detach())) <= tol * abs(float(rloss.detach()))
+        assert abs(float(norm) - float(rnorm)) <= tol * float(rnorm)
+        for p, r in zip(leaves, ref):
+            assert float((p.grad.cpu().double() - r.grad).norm()) <= tol * float(r.grad.norm())
+        assert torch.equal(top, ops.topk_rows(s.detach(), 5))
+        opt.step()
+        ropt.step()
+        with torch.no_grad():
+            for p, r in zip(leaves, ref):                     # the next step starts from the same weights
+                if t == torch.float32:
+                    assert float((p.cpu().double() - r).abs().max()) <= 2e-3
+                r.copy_(p.cpu().double() if t == torch.float32 else p.cpu().to(t).double())
+
+
+def test_catalogue_operators_in_a_captured_graph():
+    """The whole chain with its backward forms captured and replayed on new inputs, the program's own eager work between the
+    replays, two graphs and an eager call side by side: every replay gives the eager bits."""
+    from mmssl_amd import ops, optim
+    g0 = gen(61)
+    items, d, n = 700, 64, 300
+
+    def inputs(seed):
+        q = gen(seed)
+        return [torch.randn(items, d, generator=q), torch.randint(items, (n,), generator=q),
+                torch.randn(d, generator=q), torch.randint(items, (n,), generator=q)]
+
+    def chain(table, idx, w, pos):
+        with torch.enable_grad():
+            leaves = [v.detach().requires_grad_(True) for v in (table, w)]
+            rows = ops.embed_rows(leaves[0], idx, scale=2.0)
+            user = ops.layernorm_rows(rows, leaves[1])
+            s = user @ leaves[0].t()
+            logp, entropy, top_logp, top = ops.logprobs_rows(s, pos, k=5)
+            grads = list(torch.autograd.grad((logp, entropy, top_logp), leaves,
+                                             (torch.ones_like(logp), torch.ones_like(entropy), torch.ones_like(top_logp))))
+        norm = optim.clip_grads(grads, 1.0)
+        return [logp.detach(), entropy.detach(), top_logp.detach(), top, norm] + grads
+
+    stream = torch.cuda.Stream()
+    graphs = []
+    for seed in (1, 2):
+        static = [v.to(DEV) for v in inputs(seed)]
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            chain(*static)
+        torch.cuda.current_stream().wait_stream(stream)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
+            outs = chain(*static)
+        graphs.append((g, static, outs))
+    for turn in range(4):
+        for k, (g, static, outs) in enumerate(graphs):
+            fresh = [v.to(DEV) for v in inputs(10 + 2 * turn + k)]
+            for a, b in zip(static, fresh):
+                a.copy_(b)
+            g.replay()
+            want = chain(*fresh)                              # eager, between the replays
+            torch.cuda.synchronize()
+            for i, (a, b) in enumerate(zip(outs, want)):
+                assert torch.equal(a, b), (turn, k, i)
+
+
+def test_catalogue_operators_on_two_streams_at_once():
+    from mmssl_amd import ops, optim
+    g0 = gen(71)
+    table = torch.randn(5000, 64, generator=g0).to(DEV)
+    idx = torch.randint(5000, (20000,), generator=g0).to(DEV)
+    g = torch.randn(20000, 64, generator=g0).to(DEV)
+    x = torch.randn(200, 20000, generator=g0).to(DEV)
+    tg = torch.randint(20000, (200,), generator=g0).to(DEV)
+
+    def work():
+        w = table.detach().requires_grad_(True)
+        out = ops.embed_rows(w, idx)
+        (gw,) = torch.autograd.grad(out, w, g)
+        y = ops.layernorm_rows(out.detach())
+        o = ops.logprobs_rows(x, tg, k=30)
+        c = [gw.clone(), y.clone()]
+        return [gw, y, o[0], o[1], o[2], o[3], optim.clip_grads(c, 1.0)] + c
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams * 2:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(work())
+    torch.cuda.synchronize()
+    for o in got:
+        assert all(torch.equal(a, b) for a, b in zip(o, want))
