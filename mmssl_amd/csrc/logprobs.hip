@@ -104,6 +104,24 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   return r;
 }
 
+// A lower bound of the k-th largest of all entries from the maxima (as whole numbers) of the threads that hold entries, `held`
+// of them: as many threads as alternatives have a maximum that is no smaller. Each full wave of such threads finds the q-th
+// largest of its maxima by its bits, the smallest of these is the bound; 0 where there are too few threads. One value a wave.
+__device__ __forceinline__ uint32_t wave_bound(uint32_t key, int held, int k) {
+  const int w = threadIdx.x >> 6, full = max(1, held / 64), q = (k + full - 1) / full;
+  if (w >= full) return 0xffffffffu;
+  uint32_t t = 0;
+  if (q <= 64) {
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cnd = t | (1u << bit);
+      const int n = __popcll(__ballot(key >= cnd));
+      if (n >= q) t = cnd;
+      if (n == q) break;
+    }
+  }
+  return t;
+}
+
 // the k best of n pairs in LDS, in order, to out[0, k): a pair's place is the number of better ones
 template <class PUT>
 __device__ __forceinline__ void rank_pairs(const uint64_t* __restrict__ pairs, int n, int k, PUT put) {
@@ -225,19 +243,7 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
     red[2 * kWaves + w] = a;
   }
   if (TOP) {
-    // lower bound of the k-th largest value: as many threads as alternatives have a maximum that is no smaller. Each full
-    // wave of threads with columns finds the q-th largest of its threads' maxima, the smallest of these is the bound.
-    const int held = min(kBlock, (mine + N - 1) / N), full = max(1, held / 64), q = (k + full - 1) / full;
-    uint32_t t = w < full ? 0u : 0xffffffffu;
-    if (w < full && q <= 64) {
-      const uint32_t key = order_of(tm);
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t cnd = t | (1u << bit);
-        const int n = __popcll(__ballot(key >= cnd));
-        if (n >= q) t = cnd;
-        if (n == q) break;
-      }
-    }
+    const uint32_t t = wave_bound(order_of(tm), min(kBlock, (mine + N - 1) / N), k);
     if (lane == 0) bound[w] = t;
   }
   __syncthreads();
@@ -314,70 +320,81 @@ __global__ __launch_bounds__(kBlock) void lp_join_kernel(const T* __restrict__ X
   if ((threadIdx.x & 63) == 0) write_row(X + row * ldx, cols, row, r, inv_t, o);
 }
 
-// ... with alternatives: one block a row. The slices' k best are pairs of distinct numbers: the k-th largest is found by its
-// bits (64 counts at most), the k that are left are ranked.
+// ... with alternatives: one block a row. The slices' k best are pairs of distinct numbers; a bound from the threads' largest
+// leaves a few times k of them, which are ranked. Where it leaves more than kCand, the k-th largest is found by its bits.
 template <class T>
 __global__ __launch_bounds__(kBlock) void lp_join_top_kernel(const T* __restrict__ X, int64_t ldx, int64_t cols, int splits,
                                                              float c, float inv_t, int k, RowOut o,
                                                              const Sums* __restrict__ sums,
                                                              const uint64_t* __restrict__ cand) {
-  constexpr int kHold = 4096, kDirect = 256;
-  __shared__ uint64_t held[kHold];
-  __shared__ uint64_t best[kDirect];
+  constexpr int kHold = 16;            // pairs a thread keeps in registers; the rest is read again
+  __shared__ uint64_t best[kCand];
+  __shared__ uint32_t bound[kWaves];
   __shared__ int n_best;
+  __shared__ int wsum[2][kWaves];
   const int64_t row = blockIdx.x;
-  const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));
-  if (threadIdx.x == 0) {
-    write_row(X + row * ldx, cols, row, r, inv_t, o);
-    n_best = 0;
-  }
   const int64_t total = (int64_t)splits * k;
   const uint64_t* src = cand + row * total;
-  auto put = [&](int i, uint64_t p) {
+  uint64_t own[kHold];
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < kHold; ++j) {
+    const int64_t i = (int64_t)j * kBlock + threadIdx.x;
+    own[j] = i < total ? src[i] : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < kHold; ++j) most = max(most, (uint32_t)(own[j] >> 32));
+  for (int64_t i = (int64_t)kHold * kBlock + threadIdx.x; i < total; i += kBlock)
+    most = max(most, (uint32_t)(src[i] >> 32));
+  const uint32_t t = wave_bound(most, (int)min((int64_t)kBlock, total), k);
+  if ((threadIdx.x & 63) == 0) bound[threadIdx.x >> 6] = t;
+  if (threadIdx.x == 0) n_best = 0;
+  __syncthreads();
+  const uint32_t tb = min(min(bound[0], bound[1]), min(bound[2], bound[3]));
+  auto take = [&](uint64_t p, uint64_t from) {
+    if (p && p >= from) {
+      const int j = atomicAdd(&n_best, 1);
+      if (j < kCand) best[j] = p;
+    }
+  };
+  auto take_all = [&](uint64_t from) {
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) take(own[j], from);
+    for (int64_t i = (int64_t)kHold * kBlock + threadIdx.x; i < total; i += kBlock) take(src[i], from);
+  };
+  take_all((uint64_t)tb << 32);
+  const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));      // every wave for itself
+  if (threadIdx.x == 0) write_row(X + row * ldx, cols, row, r, inv_t, o);
+  __syncthreads();
+  int n = n_best;
+  if (n > kCand) {                                                          // the same on every thread
+    uint64_t from = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t cnd = from | (1ull << bit);
+      int h = 0;
+#pragma unroll
+      for (int j = 0; j < kHold; ++j) h += own[j] >= cnd;
+      for (int64_t i = (int64_t)kHold * kBlock + threadIdx.x; i < total; i += kBlock) h += src[i] >= cnd;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) h += __shfl_xor(h, m, 64);
+      if ((threadIdx.x & 63) == 0) wsum[bit & 1][threadIdx.x >> 6] = h;
+      __syncthreads();
+      const int* q = wsum[bit & 1];
+      const int above = (q[0] + q[1]) + (q[2] + q[3]);
+      if (above >= k) from = cnd;
+      if (above == k) break;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) n_best = 0;
+    __syncthreads();
+    take_all(from);
+    __syncthreads();
+    n = n_best;
+  }
+  rank_pairs(best, n, k, [&](int i, uint64_t p) {
     o.top_idx[row * k + i] = col_of(p);
     o.top_logp[row * k + i] = logp_of(val_of(p), r, inv_t);
-  };
-  if (total <= kDirect) {
-    uint64_t p = 0;
-    if ((int)threadIdx.x < total) p = src[threadIdx.x];
-    __syncthreads();
-    if (p) best[atomicAdd(&n_best, 1)] = p;
-    __syncthreads();
-    rank_pairs(best, n_best, k, put);
-    return;
-  }
-  const bool hold = total <= kHold;
-  if (hold)
-    for (int64_t i = threadIdx.x; i < total; i += kBlock) held[i] = src[i];
-  __syncthreads();
-  uint64_t t = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t cnd = t | (1ull << bit);
-    int h = 0;
-    if (hold)
-      for (int64_t i = threadIdx.x; i < total; i += kBlock) h += held[i] >= cnd;
-    else
-      for (int64_t i = threadIdx.x; i < total; i += kBlock) h += src[i] >= cnd;
-    // counts of a thread are small: the block's count is exact in fp32 too, but stays whole here
-    __shared__ int wsum[2][kWaves];
-    int ws = h;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) ws += __shfl_xor(ws, m, 64);
-    if ((threadIdx.x & 63) == 0) wsum[bit & 1][threadIdx.x >> 6] = ws;
-    __syncthreads();
-    const int n = (wsum[bit & 1][0] + wsum[bit & 1][1]) + (wsum[bit & 1][2] + wsum[bit & 1][3]);
-    if (n >= k) t = cnd;
-    if (n == k) break;
-  }
-  for (int64_t i = threadIdx.x; i < total; i += kBlock) {
-    const uint64_t p = src[i];
-    if (p && p >= t) {
-      const int j = atomicAdd(&n_best, 1);
-      if (j < kDirect) best[j] = p;
-    }
-  }
-  __syncthreads();
-  rank_pairs(best, min(n_best, kDirect), k, put);
+  });
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------

@@ -1435,10 +1435,20 @@ def _rows2d(t):
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
+_FN = {}             # C entry points by name, bound on first use
+
+
+def _first_order(name):
+    if torch.is_grad_enabled():            # the engine enables it only for create_graph=True
+        raise _lib.MmsslError("%s: the gradient is not differentiable again" % name)
+
+
 def _call(name, t, *args):
     """One C entry point on the current stream of t's device, whichever device is current."""
     dev = t.device.index
-    fn = getattr(_lib.lib(), name)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.lib(), name)
     if dev == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
@@ -1480,8 +1490,8 @@ class _EmbedRows(torch.autograd.Function):
         return _embed_fwd(table, idx, scale, pad)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _first_order("embed_rows")
         (idx,) = ctx.saved_tensors
         (rows, d), scale, pad = ctx.cfg
         g, ldg = _rows2d(g)
@@ -1529,8 +1539,8 @@ class _LayerNormRows(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _first_order("layernorm_rows")
         X, weight, stats = ctx.saved_tensors
         shape, bias_dtype = ctx.cfg
         X2, ldx = _rows2d(X)
@@ -1583,8 +1593,8 @@ def _logprobs_fwd(X, target, k, temperature, ignore_index, want_stats):
     X2, ldx = _rows2d(X)
     rows, cols = X2.shape
     lead, dev = X.shape[:-1], X.device
-    out = torch.empty((2,) + lead, dtype=torch.float32, device=dev)
-    logp, entropy = out[0], out[1]
+    logp = torch.empty(lead, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
     top_logp = torch.empty(lead + (k,), dtype=torch.float32, device=dev) if k else None
     top_idx = torch.empty(lead + (k,), dtype=torch.int64, device=dev) if k else None
     stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
@@ -1608,8 +1618,8 @@ class _LogprobsRows(torch.autograd.Function):
         return logp, entropy, top_logp, top_idx
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
+        _first_order("logprobs_rows")
         X, target, stats, top_idx = ctx.saved_tensors
         shape, k, temperature, ignore_index = ctx.cfg
         if g_logp is None and g_entropy is None and g_top is None:

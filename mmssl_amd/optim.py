@@ -9,6 +9,8 @@ Restrictions against torch.optim.AdamW (documented, enforced where they can be):
 bias corrections are evaluated in fp32 on the device (torch's default path: host double) - the difference is
 <= 1 ulp of the step size."""
 import ctypes as _ct
+import operator
+from array import array
 
 import torch
 
@@ -189,51 +191,68 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # MMSSL_
 CLIP_EPS = 1e-6                                                         # torch.nn.utils.clip_grad_norm_'s
 
 
+_dtype_of = operator.attrgetter("dtype")
+
+
 def _grad_list(grads, what):
-    """The list's C arrays (pointers, sizes, type codes) after one look at every tensor."""
-    n = len(grads)
-    kinds = {(g.dtype, g.device) if isinstance(g, torch.Tensor) and g.layout == torch.strided else None for g in grads}
-    if None in kinds:
-        raise _lib.MmsslError("%s: dense tensors expected" % what)
-    if any(d not in _DTYPES for d, _ in kinds):
-        raise _lib.MmsslError("%s: gradients must be float32, bfloat16 or float16" % what)
-    devices = {d for _, d in kinds}
-    if len(devices) > 1 or any(d.type != "cuda" for d in devices):
+    """The list's C arrays (addresses, sizes, type codes; `array` objects) after one look at every tensor, and their device."""
+    try:
+        kinds = list(map(_dtype_of, grads))
+        where = set(map(torch.Tensor.get_device, grads))
+        whole = all(map(torch.Tensor.is_contiguous, grads))
+        ptrs = array("q", map(torch.Tensor.data_ptr, grads))
+    except (TypeError, AttributeError, RuntimeError):
+        raise _lib.MmsslError("%s: dense tensors expected" % what) from None
+    if len(where) > 1 or -1 in where:
         raise _lib.MmsslError("%s: gradients must be on one CUDA (HIP) device: this package has no CPU path" % what)
-    if not all([g.is_contiguous() for g in grads]):
+    if not whole:
         raise _lib.MmsslError("%s: gradients must be contiguous" % what)
-    ptrs = (_ct.c_void_p * n)(*[g.data_ptr() for g in grads])
-    numel = (_ct.c_int64 * n)(*[g.numel() for g in grads])
-    if len(kinds) == 1:
-        dtypes = (_ct.c_int32 * n)(*([_DTYPES[grads[0].dtype]] * n))
+    numel = array("q", map(torch.Tensor.numel, grads))
+    try:
+        dtypes = array("i", map(_DTYPES.__getitem__, kinds))
+    except KeyError:
+        raise _lib.MmsslError("%s: gradients must be float32, bfloat16 or float16" % what) from None
+    return ptrs, numel, dtypes, where.pop()
+
+
+def _norm_call(name, dev, *args):
+    """One C entry point on the current stream of device `dev`: `args` around the norm's address and a workspace."""
+    count = args[-1] if name == "mmssl_grad_norm" else args[-3]
+    L = _lib.lib()
+    nb = L.mmssl_grad_norm_workspace_bytes(count)
+    at = torch.device("cuda", dev)
+    norm = torch.empty((), dtype=torch.float32, device=at)
+    ws = torch.empty(nb, dtype=torch.uint8, device=at)
+    tail = (norm.data_ptr(), ws.data_ptr(), nb, torch._C._cuda_getCurrentRawStream(dev))
+    if dev == torch._C._cuda_getDevice():
+        rc = getattr(L, name)(*args, *tail)
     else:
-        dtypes = (_ct.c_int32 * n)(*[_DTYPES[g.dtype] for g in grads])
-    return ptrs, numel, dtypes
-
-
-def _norm_call(name, dev, args_of):
-    with torch.cuda.device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        _lib.check(getattr(_lib.lib(), name)(*args_of(norm), _lib.stream_ptr()), name)
+        with torch.cuda.device(dev):
+            rc = getattr(L, name)(*args, *tail)
+    _lib.check(rc, name)
     return norm
 
 
-@torch.no_grad()
+def _at(a):
+    """The address of an array's elements (the array lives until the call returns)."""
+    return a.buffer_info()[0]
+
+
+def _twice(ptrs, numel):
+    written = [p for p, n in zip(ptrs, numel) if n]          # empty tensors may share an address
+    return len(set(written)) != len(written)
+
+
 def grad_norm(grads):
     """The 2-norm of all elements of a list of gradients together (fp32 / bf16 / fp16, mixed, any sizes) as a 0-dim fp32 device
     tensor: one launch per 96 tensors and a small one, 64-bit sums in a fixed order, nothing read back."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         raise _lib.MmsslError("grad_norm: no gradients")
-    ptrs, numel, dtypes = _grad_list(grads, "grad_norm")
-    dev = grads[0].device
-    nb = _lib.lib().mmssl_grad_norm_workspace_bytes(len(grads))
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    return _norm_call("mmssl_grad_norm", dev,
-                      lambda norm: (ptrs, numel, dtypes, len(grads), norm.data_ptr(), ws.data_ptr(), nb))
+    ptrs, numel, dtypes, dev = _grad_list(grads, "grad_norm")
+    return _norm_call("mmssl_grad_norm", dev, _at(ptrs), _at(numel), _at(dtypes), len(grads))
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm, out=None):
     """Scale a list of gradients down to the global norm `max_norm` (times min(1, max_norm / (norm + 1e-6))) and return the norm
     they had, a 0-dim fp32 device tensor. `out`: where the scaled gradients go, one tensor of the same type and number of
@@ -245,25 +264,19 @@ def clip_grads(grads, max_norm, out=None):
         raise _lib.MmsslError("clip_grads: max_norm must be a number >= 0, got %r" % (max_norm,))
     if not grads:
         raise _lib.MmsslError("clip_grads: no gradients")
-    ptrs, numel, dtypes = _grad_list(grads, "clip_grads")
-    dev = grads[0].device
+    ptrs, numel, dtypes, dev = _grad_list(grads, "clip_grads")
     if out is None:
         optrs = ptrs
     else:
         out = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(out) != len(grads):
             raise _lib.MmsslError("clip_grads: %d outputs for %d gradients" % (len(out), len(grads)))
-        optrs, onumel, odtypes = _grad_list(out, "clip_grads: out")
-        if out[0].device != dev or bytes(onumel) != bytes(numel) or bytes(odtypes) != bytes(dtypes):
+        optrs, onumel, odtypes, odev = _grad_list(out, "clip_grads: out")
+        if odev != dev or onumel != numel or odtypes != dtypes:
             raise _lib.MmsslError("clip_grads: out must match the gradients' types, sizes and device")
-    written = [p for p, n in zip(optrs, numel) if n]
-    if len(set(written)) != len(written):
+    if len(set(optrs)) != len(optrs) and _twice(optrs, numel):
         raise _lib.MmsslError("clip_grads: the same memory twice among the %s" % ("gradients" if out is None else "outputs"))
-    nb = _lib.lib().mmssl_grad_norm_workspace_bytes(len(grads))
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    return _norm_call("mmssl_clip_grads", dev,
-                      lambda norm: (ptrs, optrs, numel, dtypes, len(grads), max_norm, CLIP_EPS, norm.data_ptr(),
-                                    ws.data_ptr(), nb))
+    return _norm_call("mmssl_clip_grads", dev, _at(ptrs), _at(optrs), _at(numel), _at(dtypes), len(grads), max_norm, CLIP_EPS)
 
 
 def clip_grad_norm(parameters, max_norm):
