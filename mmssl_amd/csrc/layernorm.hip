@@ -22,7 +22,7 @@ constexpr int kMaxInRegs = 16384;
 template <class T, int LPR, int NV, bool FULL>
 struct RowTile {
   static constexpr int N = Vec<T>::N;
-  static constexpr int TPB = LPR > kBlock ? LPR : kBlock;
+  static constexpr int TPB = LPR > 64 ? LPR : kBlock;      // a row of several waves has its block to itself
   static constexpr int GPB = TPB / LPR;          // rows of a block at a time
   static constexpr int WPR = LPR > 64 ? LPR / 64 : 1;
   typedef typename Vec<T>::f32 F;
@@ -164,20 +164,25 @@ __global__ __launch_bounds__((RowTile<T, LPR, NV, FULL>::TPB)) void ln_bwd_kerne
     if (w) load_param<N>(w, pdt, Q::col(v, lig), d, W[v]);
   }
   int64_t row = (int64_t)blockIdx.x * Q::GPB + threadIdx.x / LPR;
+  constexpr bool AHEAD = NV * N <= 8;              // with 16 values a lane and 1024 lanes the next row would spill
   typename Q::R rx[NV], rg[NV];
-  if (row < rows) {
+  if (AHEAD && row < rows) {
     Q::load(X + row * ldx, d, lig, rx);
     Q::load(G + row * ldg, d, lig, rg);
   }
   for (; row < rows; row += step) {
     typename Q::F x[NV], g[NV];
     const float2 st = stats[row];
+    if (!AHEAD) {
+      Q::load(X + row * ldx, d, lig, rx);
+      Q::load(G + row * ldg, d, lig, rg);
+    }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       x[v] = to_f32<T>(rx[v]);
       g[v] = to_f32<T>(rg[v]);
     }
-    if (row + step < rows) {
+    if (AHEAD && row + step < rows) {
       Q::load(X + (row + step) * ldx, d, lig, rx);
       Q::load(G + (row + step) * ldg, d, lig, rg);
     }
@@ -245,26 +250,26 @@ __global__ __launch_bounds__((RowTile<T, LPR, NV, FULL>::TPB)) void ln_bwd_kerne
   }
 }
 
-// gw / gb from the blocks' partial sums: 64 columns a block, its 16 groups of 16 lanes take a stripe of the partials each
+// gw / gb from the blocks' partial sums: 16 columns a block, its 64 groups of 4 lanes take every 64th partial each
 __global__ __launch_bounds__(kBlock) void ln_param_kernel(const float* __restrict__ part, int nparts, int d,
                                                           void* __restrict__ gw, void* __restrict__ gb, int pdt) {
-  __shared__ float4 red[16][16];
-  const int l = threadIdx.x & 15, gidx = threadIdx.x >> 4;
+  __shared__ float4 red[64][4];
+  const int l = threadIdx.x & 3, gidx = threadIdx.x >> 2;
   const int64_t width = 2 * (int64_t)d;
-  const int64_t c = (int64_t)blockIdx.x * 64 + l * 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + l * 4;
   Vec<float>::f32 a = 0.f;
   if (c < width) {
-#pragma unroll 4
-    for (int p = gidx; p < nparts; p += 16)
-      a += load_raw<float>(part + (int64_t)p * width + c, (int)min((int64_t)4, width - c));
+    const int left = (int)min((int64_t)4, width - c);
+#pragma unroll 8
+    for (int p = gidx; p < nparts; p += 64) a += load_raw<float>(part + (int64_t)p * width + c, left);
   }
   red[gidx][l] = make_float4(a[0], a[1], a[2], a[3]);
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int64_t col = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 16) {
+    const int64_t col = (int64_t)blockIdx.x * 16 + threadIdx.x;
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) t += reinterpret_cast<const float*>(red[k])[threadIdx.x];
+    for (int k = 0; k < 64; ++k) t += reinterpret_cast<const float*>(red[k])[threadIdx.x];
     if (col < width) {
       void* out = col < d ? gw : gb;
       const int64_t j = col < d ? col : col - d;
@@ -393,30 +398,37 @@ struct Shape {
   int lpr, nv;      // lpr 0: wide
 };
 
-// up to 16 values a lane (NV vectors of 16 bytes); the fewest lanes that hold the row, no fewer than 8
-Shape shape_for(int d, int es) {
-  const int n = 16 / es, vecs = (d + n - 1) / n, most = 16 / n;      // most = vectors a lane may hold: 4 (fp32), 2
+// The fewest lanes that hold the row with `values` (16 or 8) of it a lane; what is over 1024 lanes' share doubles it.
+Shape shape_for(int d, int es, int values) {
+  const int n = 16 / es, vecs = (d + n - 1) / n;
   if (d > kMaxInRegs) return {0, 0};
-  static const int lanes[] = {8, 16, 32, 64, 256, 1024};
-  for (int l : lanes) {
+  for (int l = 8; l <= 64; l *= 2)
     if (vecs <= l) return {l, 1};
-    if (l >= 64)
-      for (int nv = 2; nv <= most; nv *= 2)
-        if (vecs <= l * nv) return {l, nv};
+  const int nv = values / n;
+  for (int l = 64; l <= 1024; l *= 2) {
+    if (values > 8 && vecs <= l * (nv / 2)) return {l, nv / 2};
+    if (vecs <= l * nv) return {l, nv};
   }
-  return {0, 0};
+  return {1024, 16 / n};
+}
+// Forward 16 values a lane, backward 8: there three more copies of them stay in registers. 65536 x 4096 bf16, 256 lanes with
+// 16 values against 512 with 8: forward 199 against 230 us, backward 345 (3 waves a SIMD) against 302 us (4).
+Shape fwd_shape(int d, int es) { return shape_for(d, es, 16); }
+Shape bwd_shape(int d, int es) { return shape_for(d, es, 8); }
+
+int tpb_of(Shape q) { return q.lpr > 64 ? q.lpr : kBlock; }
+int gpb_of(Shape q) { return q.lpr > 64 ? 1 : kBlock / q.lpr; }
+
+// Blocks of a launch over rows: `waves` of them on each of 256 CUs, no more than the rows need.
+int64_t blocks_for(int64_t rows, Shape q, int waves) {
+  return std::min<int64_t>((rows + gpb_of(q) - 1) / gpb_of(q), (int64_t)256 * waves / (tpb_of(q) / 64));
 }
 
-int gpb_of(Shape q) { return q.lpr > kBlock ? 1 : kBlock / q.lpr; }
-
-// blocks of a launch over rows: enough to fill the chip (256 CUs) `per_cu` times, no more than the rows need
-int64_t blocks_for(int64_t rows, Shape q, int64_t most) { return std::min((rows + gpb_of(q) - 1) / gpb_of(q), most); }
-
-constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 1024;
+constexpr int kFwdWaves = 16, kBwdWaves = 16;
 int64_t wide_stripes(int64_t rows) { return std::min<int64_t>(rows, 256); }
 int64_t parts_for(int64_t rows, int d, int es) {
-  const Shape q = shape_for(d, es);
-  return q.lpr ? blocks_for(rows, q, q.lpr > kBlock ? kBwdBlocks / 2 : kBwdBlocks) : wide_stripes(rows);
+  const Shape q = bwd_shape(d, es);
+  return q.lpr ? blocks_for(rows, q, kBwdWaves) : wide_stripes(rows);
 }
 
 int check_common(int dtype, int64_t rows, int d, int pdt, float eps) {
@@ -426,22 +438,31 @@ int check_common(int dtype, int64_t rows, int d, int pdt, float eps) {
   return 0;
 }
 
+// CALL(T, LPR, NV) for the shape q: vectors of 16 values, 8, 4 (rows of few vectors, fp32)
+#define LN_LANES(T, CALL, L)                          \
+  case L:                                             \
+    if (q.nv == 1) { CALL(T, L, 1); }                 \
+    else if (q.nv == 2) { CALL(T, L, 2); }            \
+    else { CALL(T, L, 4); }                           \
+    break
 #define LN_SHAPES(T, CALL)                            \
   do {                                                \
     const bool full = d % Vec<T>::N == 0;             \
-    if (q.lpr == 8) { CALL(T, 8, 1); }                \
-    else if (q.lpr == 16) { CALL(T, 16, 1); }         \
-    else if (q.lpr == 32) { CALL(T, 32, 1); }         \
-    else if (q.lpr == 64 && q.nv == 1) { CALL(T, 64, 1); }   \
-    else if (q.lpr == 64 && q.nv == 2) { CALL(T, 64, 2); }   \
-    else if (q.lpr == 64) { CALL(T, 64, 4); }                \
-    else if (q.lpr == 256 && q.nv == 1) { CALL(T, 256, 1); } \
-    else if (q.lpr == 256 && q.nv == 2) { CALL(T, 256, 2); } \
-    else if (q.lpr == 256) { CALL(T, 256, 4); }              \
-    else if (q.nv == 1) { CALL(T, 1024, 1); }                \
-    else if (q.nv == 2) { CALL(T, 1024, 2); }                \
-    else { CALL(T, 1024, 4); }                               \
+    switch (q.lpr) {                                  \
+      LN_LANES(T, CALL, 8);                           \
+      LN_LANES(T, CALL, 16);                          \
+      LN_LANES(T, CALL, 32);                          \
+      LN_LANES(T, CALL, 64);                          \
+      LN_LANES(T, CALL, 128);                         \
+      LN_LANES(T, CALL, 256);                         \
+      LN_LANES(T, CALL, 512);                         \
+      LN_LANES(T, CALL, 1024);                        \
+    }                                                 \
   } while (0)
+// the shapes that occur: one vector up to 64 lanes; above, 8 values a lane (backward) or 8 and 16 (forward); 16 at 1024 lanes
+#define LN_FWD_HAS(T, L, V) (V == 1 ? (L <= 64 || Vec<T>::N == 8) : (L >= 64 && (V * Vec<T>::N == 8 || V * Vec<T>::N == 16)))
+#define LN_BWD_HAS(T, L, V) (V == 1 ? (L <= 64 || Vec<T>::N == 8) \
+                                    : (L >= 64 && (V * Vec<T>::N == 8 || (L == 1024 && V * Vec<T>::N == 16))))
 
 }  // namespace
 
@@ -454,7 +475,7 @@ extern "C" int mmssl_layernorm_rows(const void* X, int64_t ldx, int dtype, int64
       !aligned_to(stats, 8))
     return MMSSL_E_BADARG;
   const hipStream_t s = as_stream(stream);
-  const Shape q = shape_for(d, (int)es);
+  const Shape q = fwd_shape(d, (int)es);
   if (!q.lpr) {
 #define LN_FWD_WIDE(T)                                                                                                   \
   hipLaunchKernelGGL(ln_fwd_wide_kernel<T>, dim3((unsigned)rows), dim3(kWideThreads), 0, s, (const T*)X, ldx, d, weight,  \
@@ -463,13 +484,12 @@ extern "C" int mmssl_layernorm_rows(const void* X, int64_t ldx, int dtype, int64
     MMSSL_LAUNCH_CHECK();
     return 0;
   }
-  const dim3 grid((unsigned)blocks_for(rows, q, q.lpr > kBlock ? kFwdBlocks / 4 : kFwdBlocks));
-  const dim3 block(q.lpr > kBlock ? q.lpr : kBlock);
+  const dim3 grid((unsigned)blocks_for(rows, q, kFwdWaves)), block(tpb_of(q));
 #define LN_FWD_F(T, L, V, F)                                                                                             \
   hipLaunchKernelGGL((ln_fwd_kernel<T, L, V, F>), grid, block, 0, s, (const T*)X, ldx, rows, d, weight, bias,             \
                      param_dtype, eps, (T*)Y, (float2*)stats)
 #define LN_FWD_V(T, L, V)                                          \
-  if constexpr (V * Vec<T>::N <= 16) {                             \
+  if constexpr (LN_FWD_HAS(T, L, V)) {                             \
     if (full) LN_FWD_F(T, L, V, true);                             \
     else LN_FWD_F(T, L, V, false);                                 \
   }
@@ -501,16 +521,16 @@ extern "C" int mmssl_layernorm_rows_bwd(const void* X, int64_t ldx, const void* 
                  workspace_bytes < mmssl_layernorm_rows_bwd_workspace_bytes(dtype, rows, d)))
     return MMSSL_E_WORKSPACE;
   const hipStream_t s = as_stream(stream);
-  const Shape q = shape_for(d, (int)es);
+  const Shape q = bwd_shape(d, (int)es);
   const int64_t nparts = parts_for(rows, d, (int)es);
   if (rows > 0 && q.lpr) {
-    const dim3 grid((unsigned)nparts), block(q.lpr > kBlock ? q.lpr : kBlock);
+    const dim3 grid((unsigned)nparts), block(tpb_of(q));
     float* pp = params ? part : nullptr;
 #define LN_BWD_F(T, L, V, F)                                                                                             \
   hipLaunchKernelGGL((ln_bwd_kernel<T, L, V, F>), grid, block, 0, s, (const T*)X, ldx, (const T*)G, ldg, rows, d, weight, \
                      param_dtype, (const float2*)stats, (T*)GX, pp)
 #define LN_BWD_V(T, L, V)                                          \
-  if constexpr (V * Vec<T>::N <= 16) {                             \
+  if constexpr (LN_BWD_HAS(T, L, V)) {                             \
     if (full) LN_BWD_F(T, L, V, true);                             \
     else LN_BWD_F(T, L, V, false);                                 \
   }
@@ -535,7 +555,7 @@ extern "C" int mmssl_layernorm_rows_bwd(const void* X, int64_t ldx, const void* 
     }
   }
   if (params) {
-    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)((2 * (int64_t)d + 63) / 64)), dim3(kBlock), 0, s,
+    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)((2 * (int64_t)d + 15) / 16)), dim3(kBlock), 0, s,
                        (const float*)part, (int)nparts, d, gweight, gbias, param_dtype);
     MMSSL_LAUNCH_CHECK();
   }

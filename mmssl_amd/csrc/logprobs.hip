@@ -73,14 +73,21 @@ __device__ __forceinline__ float logp_of(float x, RowStat r, float inv_t) {
   return (x - r.m) * inv_t - r.l2 * kLn2;
 }
 
+__device__ __forceinline__ int64_t target_of(const RowOut& o, int64_t row) {
+  return o.target64 ? o.target64[row] : (int64_t)o.target32[row];
+}
+// the score of the row's target; anything where it has none
 template <class T>
-__device__ __forceinline__ void write_row(const T* __restrict__ x, int64_t cols, int64_t row, RowStat r, float inv_t,
-                                          const RowOut& o) {
-  const int64_t t = o.target64 ? o.target64[row] : (int64_t)o.target32[row];
+__device__ __forceinline__ float target_score(const T* __restrict__ x, int64_t cols, int64_t row, const RowOut& o) {
+  const int64_t t = target_of(o, row);
+  return t >= 0 && t < cols ? (float)x[t] : 0.f;
+}
+__device__ __forceinline__ void write_row(float x, int64_t cols, int64_t row, RowStat r, float inv_t, const RowOut& o) {
+  const int64_t t = target_of(o, row);
   float lp;
   if (t == o.ignore) lp = 0.f;
   else if (t < 0 || t >= cols) lp = __builtin_nanf("");
-  else lp = logp_of((float)x[t], r, inv_t);
+  else lp = logp_of(x, r, inv_t);
   o.logp[row] = lp;
   o.entropy[row] = r.h;
   if (o.stats) o.stats[row] = make_float4(r.m, r.l2, r.h, 0.f);
@@ -253,7 +260,7 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
   z.a = (red[2 * kWaves] + red[2 * kWaves + 1]) + (red[2 * kWaves + 2] + red[2 * kWaves + 3]);
   const RowStat r = stat_of(z);
   if (threadIdx.x == 0) {
-    if (splits == 1) write_row(x, cols, row, r, inv_t, o);
+    if (splits == 1) write_row(target_score(x, cols, row, o), cols, row, r, inv_t, o);
     else sums[blockIdx.x] = z;
   }
   if (!TOP) return;
@@ -316,8 +323,9 @@ __global__ __launch_bounds__(kBlock) void lp_join_kernel(const T* __restrict__ X
                                                          const Sums* __restrict__ sums) {
   const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= rows) return;
+  const float at_target = target_score(X + row * ldx, cols, row, o);
   const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));
-  if ((threadIdx.x & 63) == 0) write_row(X + row * ldx, cols, row, r, inv_t, o);
+  if ((threadIdx.x & 63) == 0) write_row(at_target, cols, row, r, inv_t, o);
 }
 
 // ... with alternatives: one block a row. The slices' k best are pairs of distinct numbers; a bound from the threads' largest
@@ -335,6 +343,8 @@ __global__ __launch_bounds__(kBlock) void lp_join_top_kernel(const T* __restrict
   const int64_t row = blockIdx.x;
   const int64_t total = (int64_t)splits * k;
   const uint64_t* src = cand + row * total;
+  // everything that depends on nothing is asked for first: each is a miss
+  const float at_target = target_score(X + row * ldx, cols, row, o);
   uint64_t own[kHold];
   uint32_t most = 0;
 #pragma unroll
@@ -364,7 +374,7 @@ __global__ __launch_bounds__(kBlock) void lp_join_top_kernel(const T* __restrict
   };
   take_all((uint64_t)tb << 32);
   const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));      // every wave for itself
-  if (threadIdx.x == 0) write_row(X + row * ldx, cols, row, r, inv_t, o);
+  if (threadIdx.x == 0) write_row(at_target, cols, row, r, inv_t, o);
   __syncthreads();
   int n = n_best;
   if (n > kCand) {                                                          // the same on every thread
@@ -428,7 +438,8 @@ __global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X,
     for (int i = 0; i < k; ++i) g += gtop[row * k + i];
   const float gh = gent ? gent[row] : 0.f;
   // gx = p (a + b log2 p) away from the named columns
-  const float a = -inv_t * (g + gh * st.z), b = -inv_t * gh * kLn2;
+  // (a row without probabilities: exp2(-inf) * 0)
+  const float a = empty ? 0.f : -inv_t * (g + gh * st.z), b = empty ? 0.f : -inv_t * gh * kLn2;
   auto common = [&](float f) {
     const float q = fmaf(f - m, c, -l2);
     const float p = __builtin_amdgcn_exp2f(q);
@@ -441,7 +452,7 @@ __global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X,
       const F f = to_f32<T>(raw[v]);
       F y;
 #pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = empty ? 0.f : common(f[e]);
+      for (int e = 0; e < N; ++e) y[e] = common(f[e]);
       store_f32<T, FULL>(gx + at, (int)min((int64_t)N, cols - at), y);
     }
   }
