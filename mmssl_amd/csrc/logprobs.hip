@@ -96,18 +96,11 @@ __device__ __forceinline__ void write_row(float x, int64_t cols, int64_t row, Ro
 __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   Sums r;
   r.m = fmaxf(a.m, b.m);
-  r.s = 0.f;
-  r.a = 0.f;
-  if (a.s != 0.f) {                              // NaN counts
-    const float d = (a.m - r.m) * c, f = exp2f(d);
-    r.s += a.s * f;
-    r.a += f == 0.f ? 0.f : (a.a + d * a.s) * f;
-  }
-  if (b.s != 0.f) {
-    const float d = (b.m - r.m) * c, f = exp2f(d);
-    r.s += b.s * f;
-    r.a += f == 0.f ? 0.f : (b.a + d * b.s) * f;
-  }
+  // a side of nothing but -inf (s = 0) has no part; a NaN in s counts. Far below the other: factor 0, and 0 * -inf is kept out
+  const float da = a.s == 0.f ? kFar : fmaxf((a.m - r.m) * c, kFar), db = b.s == 0.f ? kFar : fmaxf((b.m - r.m) * c, kFar);
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  r.s = a.s * fa + b.s * fb;
+  r.a = fmaf(da, a.s, a.a) * fa + fmaf(db, b.s, b.a) * fb;
   return r;
 }
 
@@ -186,7 +179,7 @@ __device__ __attribute__((noinline)) void pick_exactly(const T* __restrict__ x, 
 
 // ---- forward: slices --------------------------------------------------------------------------------------------------
 // Block (row, slice): columns [slice * len, ...). NV vectors a thread; vector v of thread t starts at column
-// (v * kBlock + t) * N of the slice. sums [rows][splits], cand [rows][splits][k]. With one slice a row the block writes the
+// (v * kBlock + t) * N of the slice. sums [rows][splits], cand [rows][k][splits]. With one slice a row the block writes the
 // row's results itself.
 template <class T, int NV, bool FULL, bool TOP>
 __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ X, int64_t ldx, int64_t cols, int len,
@@ -232,17 +225,27 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
   __syncthreads();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float base = m == -__builtin_inff() ? 0.f : m;          // nothing but -inf (and NaN): y = -inf, e = 0
+  // y = (x - base) c as one fma around hi = base c: off by the same known lo = base c - hi in every term, which is taken
+  // out of the sums below. Scores so large that lo is no longer small are subtracted first.
+  const float hi = base * c;
+  const bool fused = fabsf(hi) <= 1048576.f;
+  const float lo = fused ? fmaf(base, c, -hi) : 0.f;
   float s = 0.f, a = 0.f;
+  auto sweep = [&](auto dist) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float y = ((float)raw[v][e] - base) * c;
-      const float p = __builtin_amdgcn_exp2f(y);
-      s += p;
-      a = fmaf(p, fmaxf(y, kFar), a);                           // a NaN is in p as well
-    }
+      for (int e = 0; e < N; ++e) {
+        const float y = dist((float)raw[v][e]);
+        const float p = __builtin_amdgcn_exp2f(y);
+        s += p;
+        a = fmaf(p, fmaxf(y, kFar), a);                         // a NaN is in p as well
+      }
+  };
+  if (fused) sweep([&](float f) { return fmaf(f, c, -hi); });
+  else sweep([&](float f) { return (f - base) * c; });
   const bool odd = s != s;                                      // this thread holds a NaN (or the row an infinity)
+  a = fmaf(-lo, s, a);
   s = group_sum<64>(s);
   a = group_sum<64>(a);
   if (lane == 0) {
@@ -256,8 +259,9 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
   __syncthreads();
   Sums z;
   z.m = m;
-  z.s = (red[kWaves] + red[kWaves + 1]) + (red[kWaves + 2] + red[kWaves + 3]);
-  z.a = (red[2 * kWaves] + red[2 * kWaves + 1]) + (red[2 * kWaves + 2] + red[2 * kWaves + 3]);
+  const float back = exp2f(-lo);
+  z.s = ((red[kWaves] + red[kWaves + 1]) + (red[kWaves + 2] + red[kWaves + 3])) * back;
+  z.a = ((red[2 * kWaves] + red[2 * kWaves + 1]) + (red[2 * kWaves + 2] + red[2 * kWaves + 3])) * back;
   const RowStat r = stat_of(z);
   if (threadIdx.x == 0) {
     if (splits == 1) write_row(target_score(x, cols, row, o), cols, row, r, inv_t, o);
@@ -269,17 +273,23 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
   // tb = 0: no bound. NaN is above every bound: !(x < tf)
   const float tf = tb == 0 ? -__builtin_inff() : value_of(tb);
   if (!(tm < tf) || odd) {
+    int mine_n = 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float f = (float)raw[v][e];
-        const int at = (v * kBlock + threadIdx.x) * N + e;
-        if (!(f < tf) && at < mine) {
-          const int i = atomicAdd(&n_pairs, 1);
-          if (i < kCand) pairs[i] = pair_of(f, c0 + at);
+      for (int e = 0; e < N; ++e)
+        mine_n += !((float)raw[v][e] < tf) && (v * kBlock + (int)threadIdx.x) * N + e < mine;
+    int i = mine_n ? atomicAdd(&n_pairs, mine_n) : kCand;         // one place for all of a thread's
+    if (i + mine_n <= kCand) {                                    // (what does not fit is picked below)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float f = (float)raw[v][e];
+          const int at = (v * kBlock + threadIdx.x) * N + e;
+          if (!(f < tf) && at < mine) pairs[i++] = pair_of(f, c0 + at);
         }
-      }
+    }
   }
   __syncthreads();
   int n = n_pairs;
@@ -294,100 +304,144 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
       o.top_logp[row * k + i] = logp_of(val_of(p), r, inv_t);
     });
   } else {
-    uint64_t* out = cand + (int64_t)blockIdx.x * k;
-    rank_pairs(pairs, n, k, [&](int i, uint64_t p) { out[i] = p; });
-    for (int i = n + threadIdx.x; i < k; i += kBlock) out[i] = 0;
+    uint64_t* out = cand + row * k * splits + slice;              // [rows][k][splits]: the slices' best, then their next ...
+    rank_pairs(pairs, n, k, [&](int i, uint64_t p) { out[(int64_t)i * splits] = p; });
+    for (int i = n + threadIdx.x; i < k; i += kBlock) out[(int64_t)i * splits] = 0;
   }
 }
 
 // ---- forward: the slices of a row -------------------------------------------------------------------------------------
-// sums of a row, by one wave; every lane ends with them. The order is fixed by the lane and the shuffles.
-__device__ __forceinline__ Sums row_sums(const Sums* __restrict__ p, int splits, float c) {
-  const int lane = threadIdx.x & 63;
-  Sums z = {-__builtin_inff(), 0.f, 0.f};
-  for (int i = lane; i < splits; i += 64) z = join(z, p[i], c);
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
+// These kernels run once through little data: what they cost is misses, of data and of instructions. What can be asked for at
+// once is, and their loops stay rolled (the same with 16 pairs a thread in unrolled registers: 20 us for one row of 1 M
+// columns, of it 9 for code that had to come from memory).
+
+// Sums of the `group` (a power of two, up to a wave) neighbouring lanes, joined in a fixed order; the first has them.
+__device__ __forceinline__ Sums join_lanes(Sums z, int group, float c) {
+#pragma unroll 1
+  for (int m = 1; m < group; m <<= 1) {
     Sums y;
     y.m = __shfl_xor(z.m, m, 64);
     y.s = __shfl_xor(z.s, m, 64);
     y.a = __shfl_xor(z.a, m, 64);
-    z = (lane & m) ? join(y, z, c) : join(z, y, c);             // the same operands in the same order on both lanes
+    const bool second = threadIdx.x & m;                          // the same operands in the same order on both lanes
+    z = join({second ? y.m : z.m, second ? y.s : z.s, second ? y.a : z.a},
+             {second ? z.m : y.m, second ? z.s : y.s, second ? z.a : y.a}, c);
   }
   return z;
 }
 
+// `group` lanes a row
 template <class T>
 __global__ __launch_bounds__(kBlock) void lp_join_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows, int64_t cols,
-                                                         int splits, float c, float inv_t, RowOut o,
+                                                         int splits, int group, float c, float inv_t, RowOut o,
                                                          const Sums* __restrict__ sums) {
-  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const float at_target = target_score(X + row * ldx, cols, row, o);
-  const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));
-  if ((threadIdx.x & 63) == 0) write_row(at_target, cols, row, r, inv_t, o);
+  const int64_t row = (int64_t)blockIdx.x * (kBlock / group) + threadIdx.x / group;
+  const int lane = threadIdx.x & (group - 1);
+  Sums z = {-__builtin_inff(), 0.f, 0.f};
+  float at_target = 0.f;
+  if (row < rows) {
+    if (lane < splits) z = sums[row * splits + lane];
+    if (lane == 0) at_target = target_score(X + row * ldx, cols, row, o);
+#pragma unroll 1
+    for (int i = lane + group; i < splits; i += group) z = join(z, sums[row * splits + i], c);
+  }
+  z = join_lanes(z, group, c);
+  if (row < rows && lane == 0) write_row(at_target, cols, row, stat_of(z), inv_t, o);
 }
 
-// ... with alternatives: one block a row. The slices' k best are pairs of distinct numbers; a bound from the threads' largest
-// leaves a few times k of them, which are ranked. Where it leaves more than kCand, the k-th largest is found by its bits.
+// ... with alternatives: one block a row. The slices' k best are pairs of distinct numbers, the slices' first ones before their
+// second ones: the k-th largest of the first 256 bounds the row's k-th largest from below and leaves a few times k pairs, which
+// are ranked. Up to `hold` pairs are all looked at (LDS); of longer lists each thread follows its slices' down to the bound.
+// Where the bound leaves more than kCand, the k-th largest is found by its bits.
 template <class T>
 __global__ __launch_bounds__(kBlock) void lp_join_top_kernel(const T* __restrict__ X, int64_t ldx, int64_t cols, int splits,
                                                              float c, float inv_t, int k, RowOut o,
                                                              const Sums* __restrict__ sums,
-                                                             const uint64_t* __restrict__ cand) {
-  constexpr int kHold = 16;            // pairs a thread keeps in registers; the rest is read again
+                                                             const uint64_t* __restrict__ cand, int hold) {
+  extern __shared__ uint64_t held[];
   __shared__ uint64_t best[kCand];
+  __shared__ Sums part[kWaves];
   __shared__ uint32_t bound[kWaves];
   __shared__ int n_best;
   __shared__ int wsum[2][kWaves];
+  constexpr int kAhead = 4;
   const int64_t row = blockIdx.x;
-  const int64_t total = (int64_t)splits * k;
+  const int tid = threadIdx.x, total = splits * k;
+  const bool flat = total <= hold;
   const uint64_t* src = cand + row * total;
-  // everything that depends on nothing is asked for first: each is a miss
-  const float at_target = target_score(X + row * ldx, cols, row, o);
-  uint64_t own[kHold];
-  uint32_t most = 0;
+  const uint64_t first = tid < total ? src[tid] : 0;
+  uint64_t next[kAhead];                             // of the thread's first slice, below its best
+  if (!flat) {
 #pragma unroll
-  for (int j = 0; j < kHold; ++j) {
-    const int64_t i = (int64_t)j * kBlock + threadIdx.x;
-    own[j] = i < total ? src[i] : 0;
+    for (int j = 0; j < kAhead; ++j) next[j] = tid < splits && j + 1 < k ? src[(j + 1) * splits + tid] : 0;
   }
-#pragma unroll
-  for (int j = 0; j < kHold; ++j) most = max(most, (uint32_t)(own[j] >> 32));
-  for (int64_t i = (int64_t)kHold * kBlock + threadIdx.x; i < total; i += kBlock)
-    most = max(most, (uint32_t)(src[i] >> 32));
-  const uint32_t t = wave_bound(most, (int)min((int64_t)kBlock, total), k);
-  if ((threadIdx.x & 63) == 0) bound[threadIdx.x >> 6] = t;
-  if (threadIdx.x == 0) n_best = 0;
+  Sums z = {-__builtin_inff(), 0.f, 0.f};
+  if (tid < splits) z = sums[row * splits + tid];
+  float at_target = 0.f;
+  if (tid == kBlock - 1) at_target = target_score(X + row * ldx, cols, row, o);
+  if (flat) {
+    if (tid < total) held[tid] = first;
+#pragma unroll 4
+    for (int i = tid + kBlock; i < total; i += kBlock) held[i] = src[i];
+  }
+#pragma unroll 1
+  for (int i = tid + kBlock; i < splits; i += kBlock) z = join(z, sums[row * splits + i], c);
+  const uint32_t t = wave_bound((uint32_t)(first >> 32), min(kBlock, total), k);
+  z = join_lanes(z, 64, c);
+  if ((tid & 63) == 0) {
+    bound[tid >> 6] = t;
+    part[tid >> 6] = z;
+  }
+  if (tid == 0) n_best = 0;
   __syncthreads();
-  const uint32_t tb = min(min(bound[0], bound[1]), min(bound[2], bound[3]));
-  auto take = [&](uint64_t p, uint64_t from) {
-    if (p && p >= from) {
-      const int j = atomicAdd(&n_best, 1);
-      if (j < kCand) best[j] = p;
+  z = part[0];
+#pragma unroll 1
+  for (int w = 1; w < kWaves; ++w) z = join(z, part[w], c);
+  const RowStat r = stat_of(z);
+  if (tid == kBlock - 1) write_row(at_target, cols, row, r, inv_t, o);
+  auto put = [&](uint64_t p) {
+    const int at = atomicAdd(&n_best, 1);
+    if (at < kCand) best[at] = p;
+  };
+  auto take = [&](uint64_t from) {                                          // from >= 1: 0 is no pair
+    if (flat) {
+#pragma unroll 1
+      for (int i = tid; i < total; i += kBlock)
+        if (held[i] >= from) put(held[i]);
+      return;
+    }
+#pragma unroll 1
+    for (int s = tid; s < splits; s += kBlock) {
+#pragma unroll 1
+      for (int j = 0; j < k; ++j) {
+        uint64_t p;
+        if (s == tid && j <= kAhead) {
+          p = first;
+#pragma unroll
+          for (int h = 0; h < kAhead; ++h)
+            if (j == h + 1) p = next[h];
+        } else {
+          p = src[(int64_t)j * splits + s];
+        }
+        if (p < from) break;
+        put(p);
+      }
     }
   };
-  auto take_all = [&](uint64_t from) {
-#pragma unroll
-    for (int j = 0; j < kHold; ++j) take(own[j], from);
-    for (int64_t i = (int64_t)kHold * kBlock + threadIdx.x; i < total; i += kBlock) take(src[i], from);
-  };
-  take_all((uint64_t)tb << 32);
-  const RowStat r = stat_of(row_sums(sums + row * splits, splits, c));      // every wave for itself
-  if (threadIdx.x == 0) write_row(at_target, cols, row, r, inv_t, o);
+  const uint32_t tb = min(min(bound[0], bound[1]), min(bound[2], bound[3]));
+  take(max((uint64_t)tb << 32, (uint64_t)1));
   __syncthreads();
   int n = n_best;
   if (n > kCand) {                                                          // the same on every thread
     uint64_t from = 0;
+#pragma unroll 1
     for (int bit = 63; bit >= 0; --bit) {
       const uint64_t cnd = from | (1ull << bit);
       int h = 0;
-#pragma unroll
-      for (int j = 0; j < kHold; ++j) h += own[j] >= cnd;
-      for (int64_t i = (int64_t)kHold * kBlock + threadIdx.x; i < total; i += kBlock) h += src[i] >= cnd;
+      for (int i = tid; i < total; i += kBlock) h += src[i] >= cnd;
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) h += __shfl_xor(h, m, 64);
-      if ((threadIdx.x & 63) == 0) wsum[bit & 1][threadIdx.x >> 6] = h;
+      if ((tid & 63) == 0) wsum[bit & 1][tid >> 6] = h;
       __syncthreads();
       const int* q = wsum[bit & 1];
       const int above = (q[0] + q[1]) + (q[2] + q[3]);
@@ -395,9 +449,9 @@ __global__ __launch_bounds__(kBlock) void lp_join_top_kernel(const T* __restrict
       if (above == k) break;
     }
     __syncthreads();
-    if (threadIdx.x == 0) n_best = 0;
+    if (tid == 0) n_best = 0;
     __syncthreads();
-    take_all(from);
+    take(max(from, (uint64_t)1));
     __syncthreads();
     n = n_best;
   }
@@ -480,10 +534,11 @@ struct Cut {
   int64_t splits;
 };
 
-// Slices as long as a block's registers hold (64 values a thread); shorter ones where that leaves fewer than 512 blocks.
-// Slices of a row are of equal length, to whole vectors.
+// Slices of 32 values a thread (with 64, two thirds of the waves fit: 8192 x 35598 bf16 forward 188 -> 150 us, 1024 x 18357 fp32
+// with 50 alternatives 34 -> 28 us); shorter ones where that leaves fewer than 512 blocks. Slices of a row are of equal length,
+// to whole vectors.
 Cut cut_for(int64_t rows, int64_t cols, int es) {
-  const int n = 16 / es, most = 64 / n;
+  const int n = 16 / es, most = 32 / n;
   Cut q{};
   for (q.nv = most; q.nv > 2; q.nv /= 2)
     if (rows * ((cols + kBlock * n * q.nv - 1) / (kBlock * n * q.nv)) >= 512) break;
@@ -505,7 +560,8 @@ int check_common(int dtype, int64_t rows, int64_t cols, int target_bytes, int k,
   if (!known_dtype(dtype) || rows < 0 || cols < 1 || (target_bytes != 4 && target_bytes != 8) || k < 0) return MMSSL_E_BADARG;
   if (!(temperature > 0.f) || temperature > 3.0e38f || !(1.0f / temperature <= 3.0e38f)) return MMSSL_E_BADARG;
   if (k > kTopMax || k > cols || cols > 0x7ffffff0) return MMSSL_E_UNSUPP;
-  if (rows * ((cols + 2047) / 2048) > 0x3fffffff) return MMSSL_E_UNSUPP;     // blocks of a launch
+  // blocks of a launch; a row's pairs (at most cols / 2048 + 1 slices of k) are counted in 32 bits
+  if (rows * ((cols + 2047) / 2048) > 0x3fffffff) return MMSSL_E_UNSUPP;
   return 0;
 }
 
@@ -542,7 +598,7 @@ extern "C" int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_
   hipLaunchKernelGGL((lp_slice_kernel<T, V, F, TOP>), grid, block, 0, s, (const T*)X, ldx, cols, q.len, (int)q.splits, c, \
                      inv_t, k, o, sums, cand)
 #define LP_SLICE_V(T, V)                                         \
-  if constexpr (V * Vec<T>::N <= 64) {                           \
+  if constexpr (V * Vec<T>::N <= 32) {                           \
     if (cols % Vec<T>::N == 0) {                                 \
       if (k) LP_SLICE_T(T, V, true, true);                       \
       else LP_SLICE_T(T, V, true, false);                        \
@@ -553,7 +609,6 @@ extern "C" int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_
   }
 #define LP_SLICE(T)                      \
   switch (q.nv) {                        \
-    case 16: LP_SLICE_V(T, 16); break;   \
     case 8: LP_SLICE_V(T, 8); break;     \
     case 4: LP_SLICE_V(T, 4); break;     \
     default: LP_SLICE_V(T, 2); break;    \
@@ -563,11 +618,14 @@ extern "C" int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_
   if (q.splits == 1) return 0;
 #define LP_JOIN(T)                                                                                                       \
   if (k)                                                                                                                 \
-    hipLaunchKernelGGL(lp_join_top_kernel<T>, dim3((unsigned)rows), block, 0, s, (const T*)X, ldx, cols, (int)q.splits, c, \
-                       inv_t, k, o, (const Sums*)sums, (const uint64_t*)cand);                                           \
+    hipLaunchKernelGGL(lp_join_top_kernel<T>, dim3((unsigned)rows), block, (size_t)hold * 8, s, (const T*)X, ldx, cols,   \
+                       (int)q.splits, c, inv_t, k, o, (const Sums*)sums, (const uint64_t*)cand, hold);                   \
   else                                                                                                                   \
-    hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)((rows + kWaves - 1) / kWaves)), block, 0, s, (const T*)X, ldx,  \
-                       rows, cols, (int)q.splits, c, inv_t, o, (const Sums*)sums)
+    hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)((rows * group + kBlock - 1) / kBlock)), block, 0, s,            \
+                       (const T*)X, ldx, rows, cols, (int)q.splits, group, c, inv_t, o, (const Sums*)sums)
+  const int hold = (int)std::min<int64_t>(q.splits * k, 2048);              // pairs in LDS: 16 KB at most
+  int group = 1;
+  while (group < 64 && group < q.splits) group *= 2;
   MMSSL_BY_DTYPE(dtype, LP_JOIN);
   MMSSL_LAUNCH_CHECK();
   return 0;
