@@ -251,6 +251,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_binding = None
 
 
 class MmsslError(RuntimeError):
@@ -278,6 +279,23 @@ def lib():
         raise MmsslError("libmmssl_hip.so ABI version mismatch")
     _lib = L
     return L
+
+
+def binding():
+    """The native binding of the operators that are called often on little data (csrc/torch_binding.cpp), bound to this
+    process's lib(). Raises if it has not been built."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    L = lib()
+    try:
+        from . import _torch_binding as b
+    except ImportError as e:
+        raise MmsslError("mmssl_amd/_torch_binding.so: %s — the native binding is required (no fallback path). "
+                         "Run `python -m mmssl_amd.build`." % e) from e
+    b.bind(L._handle, MmsslError)
+    _binding = b
+    return b
 
 
 def check(code, what):

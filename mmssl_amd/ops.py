@@ -1408,99 +1408,20 @@ def ngcf_combine(G, B, keep=None, scale=1.0):
 
 
 # ---------------------------------------------------------------------------------------
-# Operators of a full-catalogue softmax model (csrc/embed.hip, layernorm.hip, logprobs.hip): fp32, bf16 and fp16
+# Operators of a full-catalogue softmax model (csrc/embed.hip, layernorm.hip, logprobs.hip): fp32, bf16 and fp16. Checks,
+# output tensors and autograd nodes are in csrc/torch_binding.cpp.
 # ---------------------------------------------------------------------------------------
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # MMSSL_F32 / BF16 / F16
-
-
-def _typed(t, name):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+def _given(t, name):
+    if not isinstance(t, torch.Tensor):
         raise _lib.MmsslError("%s must be a CUDA (HIP) tensor: this package has no CPU path" % name)
-    if t.dtype not in _DTYPES:
-        raise _lib.MmsslError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    return _DTYPES[t.dtype]
 
 
-def _same_device(t, other, name):
-    if other.device != t.device:
-        raise _lib.MmsslError("%s is on %s, expected %s" % (name, other.device, t.device))
-
-
-def _rows2d(t):
-    """(t as [rows, d] with unit column stride, row pitch): a view where the strides allow it."""
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
-
-
-_FN = {}             # C entry points by name, bound on first use
-
-
-def _first_order(name):
-    if torch.is_grad_enabled():            # the engine enables it only for create_graph=True
-        raise _lib.MmsslError("%s: the gradient is not differentiable again" % name)
-
-
-def _call(name, t, *args):
-    """One C entry point on the current stream of t's device, whichever device is current."""
-    dev = t.device.index
-    fn = _FN.get(name)
-    if fn is None:
-        fn = _FN[name] = getattr(_lib.lib(), name)
-    if dev == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        _lib.check(rc, name)
-
-
-def _tokens(idx, name, device):
-    """int32 / int64 numbers on `device`, contiguous (lists and host tensors are uploaded like ops._idx does)."""
-    if not isinstance(idx, torch.Tensor):
-        idx = torch.as_tensor(idx)
-        if idx.numel() == 0:
-            idx = idx.to(torch.int64)
-    if idx.dtype not in (torch.int64, torch.int32):
-        raise _lib.MmsslError("%s must hold int64 or int32 numbers, got %s" % (name, idx.dtype))
-    if idx.device != device:
-        if idx.is_cuda:
-            raise _lib.MmsslError("%s is on %s, expected %s" % (name, idx.device, device))
-        idx = idx.to(device)
-    return idx if idx.is_contiguous() else idx.contiguous()
-
-
-def _embed_fwd(table, idx, scale, pad):
-    rows, d = table.shape
-    out = torch.empty(idx.shape + (d,), dtype=table.dtype, device=table.device)
-    ldt = table.stride(0) if rows > 1 else d
-    _call("mmssl_embed_rows", table, table.data_ptr(), ldt, _DTYPES[table.dtype], rows, d, idx.data_ptr(), idx.element_size(),
-          idx.numel(), scale, pad is not None, pad or 0, out.data_ptr(), d)
-    return out
-
-
-class _EmbedRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, idx, scale, pad):
-        ctx.save_for_backward(idx)
-        ctx.cfg = (table.shape, scale, pad)
-        return _embed_fwd(table, idx, scale, pad)
-
-    @staticmethod
-    def backward(ctx, g):
-        _first_order("embed_rows")
-        (idx,) = ctx.saved_tensors
-        (rows, d), scale, pad = ctx.cfg
-        g, ldg = _rows2d(g)
-        grad = torch.empty((rows, d), dtype=g.dtype, device=g.device)
-        nb = _lib.lib().mmssl_embed_rows_bwd_workspace_bytes(rows, d, idx.numel())
-        ws = torch.empty(nb, dtype=torch.uint8, device=g.device)
-        _call("mmssl_embed_rows_bwd", g, g.data_ptr(), ldg, _DTYPES[g.dtype], idx.data_ptr(), idx.element_size(), idx.numel(),
-              rows, d, scale, pad is not None, pad or 0, grad.data_ptr(), ws.data_ptr(), nb)
-        return grad, None, None, None
+def _numbers(idx):
+    """A tensor of whole numbers out of a list or an array (empty ones have no type of their own)."""
+    if isinstance(idx, torch.Tensor):
+        return idx
+    idx = torch.as_tensor(idx)
+    return idx if idx.numel() else idx.to(torch.int64)
 
 
 def embed_rows(table, idx, scale=1.0, padding_idx=None):
@@ -1509,129 +1430,16 @@ def embed_rows(table, idx, scale=1.0, padding_idx=None):
     of zeros; any other token outside the table gives a row of NaN. Differentiable in `table`: the dense [rows, d] gradient
     adds equal tokens in the order of their places with fp32 sums (the same call gives the same bits); padding and tokens
     outside the table add nothing."""
-    _typed(table, "table")
-    if table.dim() != 2 or table.shape[1] < 1 or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise _lib.MmsslError("embed_rows: table must be [rows, d] with unit column stride")
-    idx = _tokens(idx, "idx", table.device)
-    pad = None if padding_idx is None else int(padding_idx)
-    if table.requires_grad and torch.is_grad_enabled():
-        return _EmbedRows.apply(table, idx, float(scale), pad)
-    return _embed_fwd(table, idx, float(scale), pad)
-
-
-def _layernorm_fwd(X, weight, bias, eps, want_stats):
-    X2, ldx = _rows2d(X)
-    rows, d = X2.shape
-    y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=X.device) if want_stats else None
-    p = weight if weight is not None else bias
-    _call("mmssl_layernorm_rows", X, X2.data_ptr(), ldx, _DTYPES[X.dtype], rows, d, _ptr(weight), _ptr(bias),
-          0 if p is None else _DTYPES[p.dtype], eps, y.data_ptr(), _ptr(stats))
-    return y, X2, stats
-
-
-class _LayerNormRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, X, weight, bias, eps):
-        y, X2, stats = _layernorm_fwd(X, weight, bias, eps, True)
-        ctx.save_for_backward(X2 if X.dim() != 2 else X, weight, stats)
-        ctx.cfg = (X.shape, None if bias is None else bias.dtype)
-        return y
-
-    @staticmethod
-    def backward(ctx, g):
-        _first_order("layernorm_rows")
-        X, weight, stats = ctx.saved_tensors
-        shape, bias_dtype = ctx.cfg
-        X2, ldx = _rows2d(X)
-        rows, d = X2.shape
-        g, ldg = _rows2d(g)
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        gx = torch.empty(shape, dtype=X2.dtype, device=X2.device) if want_x else None
-        pdt = weight.dtype if weight is not None else bias_dtype if bias_dtype is not None else X2.dtype
-        gw = torch.empty(d, dtype=pdt, device=X2.device) if want_w else None
-        gb = torch.empty(d, dtype=pdt, device=X2.device) if want_b else None
-        nb = _lib.lib().mmssl_layernorm_rows_bwd_workspace_bytes(_DTYPES[X2.dtype], rows, d) if want_w or want_b else 0
-        ws = torch.empty(nb, dtype=torch.uint8, device=X2.device) if nb else None
-        _call("mmssl_layernorm_rows_bwd", X2, X2.data_ptr(), ldx, g.data_ptr(), ldg, _DTYPES[X2.dtype], rows, d, _ptr(weight),
-              _DTYPES[pdt], stats.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nb)
-        return gx, gw, gb, None
+    _given(table, "table")
+    return _lib.binding().embed_rows(table, _numbers(idx), scale, padding_idx)
 
 
 def layernorm_rows(X, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension: (x - mean) / sqrt(var + eps) * weight + bias, fp32 / bf16 / fp16 with fp32 means
     and variances, rounded once. `weight` / `bias`: [d] tensors of X's type or fp32 (both of one type), or None.
     Differentiable in X, weight and bias; the parameters' sums over the rows are fp32 in a fixed order."""
-    _typed(X, "X")
-    if X.dim() < 1 or X.shape[-1] < 1:
-        raise _lib.MmsslError("layernorm_rows: X must be [..., d] with d >= 1")
-    if not 0.0 <= eps < float("inf"):
-        raise _lib.MmsslError("layernorm_rows: eps must be a finite number >= 0, got %r" % (eps,))
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        _typed(p, name)
-        _same_device(X, p, name)
-        if p.dim() != 1 or p.shape[0] != X.shape[-1]:
-            raise _lib.MmsslError("layernorm_rows: %s must be [%d], got %s" % (name, X.shape[-1], tuple(p.shape)))
-        if p.dtype != X.dtype and p.dtype != torch.float32:
-            raise _lib.MmsslError("layernorm_rows: %s must be %s or float32, got %s" % (name, X.dtype, p.dtype))
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise _lib.MmsslError("layernorm_rows: weight and bias must be of one type")
-    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    if torch.is_grad_enabled() and (X.requires_grad or (w is not None and w.requires_grad)
-                                    or (b is not None and b.requires_grad)):
-        return _LayerNormRows.apply(X, w, b, float(eps))
-    return _layernorm_fwd(X, w, b, float(eps), False)[0]
-
-
-LOGPROBS_MAX_K = 128
-
-
-def _logprobs_fwd(X, target, k, temperature, ignore_index, want_stats):
-    X2, ldx = _rows2d(X)
-    rows, cols = X2.shape
-    lead, dev = X.shape[:-1], X.device
-    logp = torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    top_logp = torch.empty(lead + (k,), dtype=torch.float32, device=dev) if k else None
-    top_idx = torch.empty(lead + (k,), dtype=torch.int64, device=dev) if k else None
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
-    dt = _DTYPES[X.dtype]
-    nb = _lib.lib().mmssl_logprobs_rows_workspace_bytes(dt, rows, cols, k)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    _call("mmssl_logprobs_rows", X, X2.data_ptr(), ldx, dt, rows, cols, target.data_ptr(), target.element_size(), ignore_index,
-          k, temperature, logp.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_idx), _ptr(stats), ws.data_ptr(), nb)
-    return logp, entropy, top_logp, top_idx, X2, stats
-
-
-class _LogprobsRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, X, target, k, temperature, ignore_index):
-        logp, entropy, top_logp, top_idx, X2, stats = _logprobs_fwd(X, target, k, temperature, ignore_index, True)
-        ctx.save_for_backward(X2 if X.dim() != 2 else X, target, stats, top_idx)
-        ctx.cfg = (X.shape, k, temperature, ignore_index)
-        ctx.set_materialize_grads(False)
-        if top_idx is not None:
-            ctx.mark_non_differentiable(top_idx)
-        return logp, entropy, top_logp, top_idx
-
-    @staticmethod
-    def backward(ctx, g_logp, g_entropy, g_top, _):
-        _first_order("logprobs_rows")
-        X, target, stats, top_idx = ctx.saved_tensors
-        shape, k, temperature, ignore_index = ctx.cfg
-        if g_logp is None and g_entropy is None and g_top is None:
-            return None, None, None, None, None
-        X2, ldx = _rows2d(X)
-        rows, cols = X2.shape
-        g_logp, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top))
-        gx = torch.empty(shape, dtype=X2.dtype, device=X2.device)
-        _call("mmssl_logprobs_rows_bwd", X2, X2.data_ptr(), ldx, _DTYPES[X2.dtype], rows, cols, target.data_ptr(),
-              target.element_size(), ignore_index, k, temperature, _ptr(top_idx), stats.data_ptr(), _ptr(g_logp),
-              _ptr(g_entropy), _ptr(g_top), gx.data_ptr())
-        return gx, None, None, None, None
+    _given(X, "X")
+    return _lib.binding().layernorm_rows(X, weight, bias, eps)
 
 
 def logprobs_rows(X, target, k=0, temperature=1.0, ignore_index=-100):
@@ -1642,18 +1450,5 @@ def logprobs_rows(X, target, k=0, temperature=1.0, ignore_index=-100):
     Masked columns hold -inf: probability 0. A row of nothing else has logp -inf, entropy 0, gradient 0. `ignore_index` as a
     target: logp 0 and no gradient from it; any other target outside the row: logp NaN. A NaN or +inf in a row makes its logp
     and entropy NaN. Differentiable in X through logp, entropy and top_logp."""
-    _typed(X, "X")
-    k = int(k)
-    if X.dim() < 1 or X.shape[-1] < 1:
-        raise _lib.MmsslError("logprobs_rows: X must be [..., n] with n >= 1")
-    if k < 0 or k > LOGPROBS_MAX_K or k > X.shape[-1]:
-        raise _lib.MmsslError("logprobs_rows: 0 <= k <= min(%d, n) expected, got %d" % (LOGPROBS_MAX_K, k))
-    temperature = float(temperature)
-    if not 1e-30 <= temperature <= 1e30:
-        raise _lib.MmsslError("logprobs_rows: temperature must be a positive number, got %r" % (temperature,))
-    target = _tokens(target, "target", X.device)
-    if target.shape != X.shape[:-1]:
-        raise _lib.MmsslError("logprobs_rows: target must be %s, got %s" % (list(X.shape[:-1]), list(target.shape)))
-    if X.requires_grad and torch.is_grad_enabled():
-        return _LogprobsRows.apply(X, target, k, temperature, int(ignore_index))
-    return _logprobs_fwd(X, target, k, temperature, int(ignore_index), False)[:4]
+    _given(X, "X")
+    return _lib.binding().logprobs_rows(X, _numbers(target), k, temperature, ignore_index)

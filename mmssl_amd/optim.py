@@ -9,8 +9,6 @@ Restrictions against torch.optim.AdamW (documented, enforced where they can be):
 bias corrections are evaluated in fp32 on the device (torch's default path: host double) - the difference is
 <= 1 ulp of the step size."""
 import ctypes as _ct
-import operator
-from array import array
 
 import torch
 
@@ -187,96 +185,26 @@ class FusedAdamW(torch.optim.Optimizer):
 # ---------------------------------------------------------------------------------------
 # global gradient norm and clipping (csrc/gradnorm.hip)
 # ---------------------------------------------------------------------------------------
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # MMSSL_F32 / BF16 / F16
 CLIP_EPS = 1e-6                                                         # torch.nn.utils.clip_grad_norm_'s
 
 
-_dtype_of = operator.attrgetter("dtype")
-
-
-def _grad_list(grads, what):
-    """The list's C arrays (addresses, sizes, type codes; `array` objects) after one look at every tensor, and their device."""
-    try:
-        kinds = list(map(_dtype_of, grads))
-        where = set(map(torch.Tensor.get_device, grads))
-        whole = all(map(torch.Tensor.is_contiguous, grads))
-        ptrs = array("q", map(torch.Tensor.data_ptr, grads))
-    except (TypeError, AttributeError, RuntimeError):
-        raise _lib.MmsslError("%s: dense tensors expected" % what) from None
-    if len(where) > 1 or -1 in where:
-        raise _lib.MmsslError("%s: gradients must be on one CUDA (HIP) device: this package has no CPU path" % what)
-    if not whole:
-        raise _lib.MmsslError("%s: gradients must be contiguous" % what)
-    numel = array("q", map(torch.Tensor.numel, grads))
-    try:
-        dtypes = array("i", map(_DTYPES.__getitem__, kinds))
-    except KeyError:
-        raise _lib.MmsslError("%s: gradients must be float32, bfloat16 or float16" % what) from None
-    return ptrs, numel, dtypes, where.pop()
-
-
-def _norm_call(name, dev, *args):
-    """One C entry point on the current stream of device `dev`: `args` around the norm's address and a workspace."""
-    count = args[-1] if name == "mmssl_grad_norm" else args[-3]
-    L = _lib.lib()
-    nb = L.mmssl_grad_norm_workspace_bytes(count)
-    at = torch.device("cuda", dev)
-    norm = torch.empty((), dtype=torch.float32, device=at)
-    ws = torch.empty(nb, dtype=torch.uint8, device=at)
-    tail = (norm.data_ptr(), ws.data_ptr(), nb, torch._C._cuda_getCurrentRawStream(dev))
-    if dev == torch._C._cuda_getDevice():
-        rc = getattr(L, name)(*args, *tail)
-    else:
-        with torch.cuda.device(dev):
-            rc = getattr(L, name)(*args, *tail)
-    _lib.check(rc, name)
-    return norm
-
-
-def _at(a):
-    """The address of an array's elements (the array lives until the call returns)."""
-    return a.buffer_info()[0]
-
-
-def _twice(ptrs, numel):
-    written = [p for p, n in zip(ptrs, numel) if n]          # empty tensors may share an address
-    return len(set(written)) != len(written)
+def _grads(grads):
+    return [grads] if isinstance(grads, torch.Tensor) else list(grads)
 
 
 def grad_norm(grads):
     """The 2-norm of all elements of a list of gradients together (fp32 / bf16 / fp16, mixed, any sizes) as a 0-dim fp32 device
     tensor: one launch per 96 tensors and a small one, 64-bit sums in a fixed order, nothing read back."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if not grads:
-        raise _lib.MmsslError("grad_norm: no gradients")
-    ptrs, numel, dtypes, dev = _grad_list(grads, "grad_norm")
-    return _norm_call("mmssl_grad_norm", dev, _at(ptrs), _at(numel), _at(dtypes), len(grads))
+    return _lib.binding().grad_norm(_grads(grads))
 
 
 def clip_grads(grads, max_norm, out=None):
     """Scale a list of gradients down to the global norm `max_norm` (times min(1, max_norm / (norm + 1e-6))) and return the norm
     they had, a 0-dim fp32 device tensor. `out`: where the scaled gradients go, one tensor of the same type and number of
-    elements per gradient (default: the gradients themselves; no two tensors may overlap otherwise). The factor never leaves
-    the device; a NaN among the gradients makes all of them NaN, an infinite norm the finite ones 0."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise _lib.MmsslError("clip_grads: max_norm must be a number >= 0, got %r" % (max_norm,))
-    if not grads:
-        raise _lib.MmsslError("clip_grads: no gradients")
-    ptrs, numel, dtypes, dev = _grad_list(grads, "clip_grads")
-    if out is None:
-        optrs = ptrs
-    else:
-        out = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(out) != len(grads):
-            raise _lib.MmsslError("clip_grads: %d outputs for %d gradients" % (len(out), len(grads)))
-        optrs, onumel, odtypes, odev = _grad_list(out, "clip_grads: out")
-        if odev != dev or onumel != numel or odtypes != dtypes:
-            raise _lib.MmsslError("clip_grads: out must match the gradients' types, sizes and device")
-    if len(set(optrs)) != len(optrs) and _twice(optrs, numel):
-        raise _lib.MmsslError("clip_grads: the same memory twice among the %s" % ("gradients" if out is None else "outputs"))
-    return _norm_call("mmssl_clip_grads", dev, _at(ptrs), _at(optrs), _at(numel), _at(dtypes), len(grads), max_norm, CLIP_EPS)
+    elements per gradient (default: the gradients themselves). What is written may overlap nothing else. The factor never
+    leaves the device; a NaN among the gradients makes all of them NaN, an infinite norm the finite ones 0."""
+    return _lib.binding().clip_grads(_grads(grads), max_norm, CLIP_EPS,
+                                     None if out is None else _grads(out))
 
 
 def clip_grad_norm(parameters, max_norm):
