@@ -790,9 +790,9 @@ int mmssl_logprobs_rows_bwd(const void* X, int64_t ldx, int dtype, int64_t rows,
  * dtypes[i] (the arrays are host memory and read during the call): norm[0] = sqrt(sum of all squares), summed in 64 bits in a
  * fixed order; mmssl_clip_grads also writes outs[i] = grads[i] * min(1, max_norm / (norm + eps)), rounded once. outs[i] may be
  * grads[i] itself; otherwise no output may overlap a gradient or another output. The factor stays on the device: a NaN among
- * the gradients makes all of them NaN, an infinite norm makes the finite ones 0. The workspace (8-byte aligned) need not be
+ * the gradients makes all of them NaN, an infinite norm makes the finite ones 0. The workspace (16-byte aligned) need not be
  * cleared. */
-#define MMSSL_CLIP_MAX_TENSORS 96     /* of one launch; longer lists take several */
+#define MMSSL_CLIP_MAX_TENSORS 96     /* as kernel arguments; longer lists go through a table in the workspace */
 size_t mmssl_grad_norm_workspace_bytes(int count);
 int mmssl_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int count, float* norm,
                     void* workspace, size_t workspace_bytes, void* stream);

@@ -73,11 +73,12 @@ __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(const T* __restrict__
 }
 
 // ---- places by token ------------------------------------------------------------------------------------------------
+// KP: (key, place) pairs, one 8-byte access each.
 // n <= kRankMax: a place's position in the sorted list is the number of places before it, (key, place) compared as a pair.
 // One block ranks 64 places (a lane each), its 16 waves count a sixteenth of the list each.
 template <class I>
 __global__ __launch_bounds__(kSortThreads) void embed_rank_kernel(const I* __restrict__ idx, int n, IdxRule q,
-                                                                  int* __restrict__ K, int* __restrict__ P) {
+                                                                  int2* __restrict__ KP) {
   __shared__ int4 keys4[kRankTile / 4];
   __shared__ int cnt[64];
   int* keys = reinterpret_cast<int*>(keys4);
@@ -117,14 +118,13 @@ __global__ __launch_bounds__(kSortThreads) void embed_rank_kernel(const I* __res
   __syncthreads();
   if (w == 0 && i < n) {
     const int r = cnt[lane];
-    K[r] = mine;
-    P[r] = i;
+    KP[r] = make_int2(mine, i);
   }
 }
 
 // Radix passes of up to 8 bits from the low end; block b owns the places [b * per, (b + 1) * per).
 template <class I>
-__global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(const I* __restrict__ idx, const int* __restrict__ Kin,
+__global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(const I* __restrict__ idx, const int2* __restrict__ in,
                                                                   int64_t n, IdxRule q, int64_t per, int shift, int mask,
                                                                   int* __restrict__ H) {
   __shared__ int h[256];
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(const I* __res
   __syncthreads();
   const int64_t a = (int64_t)blockIdx.x * per, b = min(n, a + per);
   for (int64_t i = a + threadIdx.x; i < b; i += kSortThreads) {
-    const int k = Kin ? Kin[i] : key_of(idx[i], q);
+    const int k = in ? in[i].x : key_of(idx[i], q);
     atomicAdd(&h[(k >> shift) & mask], 1);
   }
   __syncthreads();
@@ -140,23 +140,32 @@ __global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(const I* __res
 }
 
 template <class I, int ITEMS>
-__global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(const I* __restrict__ idx, const int* __restrict__ Kin,
-                                                                     const int* __restrict__ Pin, int64_t n, IdxRule q,
-                                                                     int64_t per, int shift, int mask,
-                                                                     const int* __restrict__ H, int* __restrict__ K,
-                                                                     int* __restrict__ P) {
+__global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(const I* __restrict__ idx, const int2* __restrict__ in,
+                                                                     int64_t n, IdxRule q, int64_t per, int shift, int mask,
+                                                                     const int* __restrict__ H, int2* __restrict__ out) {
   constexpr int kWaves = kSortThreads / 64, kTile = kSortThreads * ITEMS;
   __shared__ int wc[kWaves][256];      // counts, then the next place of a wave's run of a digit
   __shared__ int base[256];
   __shared__ int wsum[4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t a = (int64_t)blockIdx.x * per, b = min(n, a + per);
+  int2 e[ITEMS];                       // (key, place); key -1: behind the block's places
+  auto load = [&](int64_t t0) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const int64_t i = t0 + (int64_t)w * 64 * ITEMS + j * 64 + lane;
+      e[j] = make_int2(-1, 0);
+      if (i < b) e[j] = in ? in[i] : make_int2(key_of(idx[i], q), (int)i);
+    }
+  };
+  load(a);                             // the first tile arrives under the counts
   // where this block's run of each digit begins: all smaller digits + this digit in the blocks before
   {
     const int dig = tid & 255, part = tid >> 8, nb = gridDim.x;
-    const int a = part * nb / 4, b = (part + 1) * nb / 4;
+    const int k0 = part * nb / 4, k1 = (part + 1) * nb / 4;
     int tot = 0, pre = 0;
 #pragma unroll 16
-    for (int k = a; k < b; ++k) {
+    for (int k = k0; k < k1; ++k) {
       const int c = H[(int64_t)k * 256 + dig];
       tot += c;
       pre += k < (int)blockIdx.x ? c : 0;
@@ -183,25 +192,15 @@ __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(const I* __
     for (int k = 0; k < w; ++k) add += wsum[k];
     base[tid] += add;
   }
-  const int64_t a = (int64_t)blockIdx.x * per, b = min(n, a + per);
   for (int64_t t0 = a; t0 < b; t0 += kTile) {
     __syncthreads();
     for (int k = tid; k < kWaves * 256; k += kSortThreads) wc[k >> 8][k & 255] = 0;
     __syncthreads();
-    int key[ITEMS], pos[ITEMS], off[ITEMS];
+    int off[ITEMS];
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
-      const int64_t i = t0 + (int64_t)w * 64 * ITEMS + j * 64 + lane;
-      key[j] = -1;
-      if (i < b) {
-        key[j] = Kin ? Kin[i] : key_of(idx[i], q);
-        pos[j] = Pin ? Pin[i] : (int)i;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-      const int dig = (key[j] >> shift) & mask;
-      uint64_t m = __ballot(key[j] >= 0);
+      const int dig = (e[j].x >> shift) & mask;
+      uint64_t m = __ballot(e[j].x >= 0);
 #pragma unroll
       for (int bit = 0; bit < 8; ++bit) {
         const uint64_t on = __ballot((dig >> bit) & 1);
@@ -209,7 +208,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(const I* __
       }
       const int before = __popcll(m & ((1ull << lane) - 1));
       int old = 0;
-      if (key[j] >= 0 && before == 0) old = atomicAdd(&wc[w][dig], __popcll(m));
+      if (e[j].x >= 0 && before == 0) old = atomicAdd(&wc[w][dig], __popcll(m));
       // lanes without a key have an empty mask: any source lane will do
       off[j] = __shfl(old, m ? __ffsll((unsigned long long)m) - 1 : 0, 64) + before;
     }
@@ -227,22 +226,19 @@ __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(const I* __
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j)
-      if (key[j] >= 0) {
-        const int to = wc[w][(key[j] >> shift) & mask] + off[j];
-        K[to] = key[j];
-        P[to] = pos[j];
-      }
+      if (e[j].x >= 0) out[wc[w][(e[j].x >> shift) & mask] + off[j]] = e[j];
+    if (t0 + kTile < b) load(t0 + kTile);
   }
 }
 
 // ---- sums of equal tokens -------------------------------------------------------------------------------------------
-// first place in the sorted K[0, n) whose key is >= x; 256 probes a round, three rounds for 16 M places
-__device__ __forceinline__ int64_t block_lower_bound(const int* __restrict__ K, int64_t n, int x) {
+// first place in the sorted KP[0, n) whose key is >= x; 256 probes a round, three rounds for 16 M places
+__device__ __forceinline__ int64_t block_lower_bound(const int2* __restrict__ KP, int64_t n, int x) {
   int64_t lo = 0, hi = n;
   while (lo < hi) {
     const int64_t s = (hi - lo + kBlock - 1) / kBlock;
     const int64_t p = lo + (threadIdx.x + 1) * s - 1;
-    const int c = __syncthreads_count(p < hi && K[p] < x);
+    const int c = __syncthreads_count(p < hi && KP[p].x < x);
     lo += c * s;
     hi = min(hi, lo + s - 1);
   }
@@ -254,7 +250,7 @@ __device__ __forceinline__ int64_t block_lower_bound(const int* __restrict__ K, 
 // part = [2][chunks][d] fp32: the sum of a chunk's first token where it began before the chunk, and of its last token where
 // that began in the chunk and goes on behind it.
 template <class T, int LPR, bool FULL>
-__global__ __launch_bounds__(kBlock) void embed_grad_kernel(const int* __restrict__ K, const int* __restrict__ P, int64_t n,
+__global__ __launch_bounds__(kBlock) void embed_grad_kernel(const int2* __restrict__ KP, int64_t n,
                                                             int rows, int d, const T* __restrict__ g, int64_t ldg,
                                                             float scale, T* __restrict__ gW, float* __restrict__ part,
                                                             int chunk, int64_t chunks, int ctiles, int64_t rblocks,
@@ -269,18 +265,17 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(const int* __restric
     const int left = d - col;
     if (left <= 0) return;
     const int64_t a = w * chunk, b = min(n, a + chunk);
-    int cur = K[a];
+    int cur = KP[a].x;
     if (cur >= rows) return;                       // the keys without a row come last
-    bool head = a > 0 && K[a - 1] == cur;
+    bool head = a > 0 && KP[a - 1].x == cur;
     F acc = 0.f;
     for (int64_t p0 = a; p0 < b; p0 += B) {
       int key[B], pos[B];
 #pragma unroll
-      for (int u = 0; u < B; u += 4) {             // K and P are padded to whole batches; chunks start at multiples of B
-        const int4 k4 = *reinterpret_cast<const int4*>(K + p0 + u);
-        const int4 p4 = *reinterpret_cast<const int4*>(P + p0 + u);
-        key[u] = k4.x; key[u + 1] = k4.y; key[u + 2] = k4.z; key[u + 3] = k4.w;
-        pos[u] = p4.x; pos[u + 1] = p4.y; pos[u + 2] = p4.z; pos[u + 3] = p4.w;
+      for (int u = 0; u < B; u += 2) {             // KP is padded to whole batches; chunks start at multiples of B
+        const int4 two = *reinterpret_cast<const int4*>(KP + p0 + u);
+        key[u] = two.x; pos[u] = two.y;
+        key[u + 1] = two.z; pos[u + 1] = two.w;
       }
       typename Vec<T>::raw v[B];
 #pragma unroll
@@ -302,7 +297,7 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(const int* __restric
         }
       }
     }
-    const bool on = b < n && K[b] == cur;
+    const bool on = b < n && KP[b].x == cur;
     if (head) store_part<N, FULL>(part + w * d + col, left, acc);
     else if (on) store_part<N, FULL>(part + (chunks + w) * d + col, left, acc);
     else store_f32<T, FULL>(gW + (int64_t)cur * d + col, left, acc * scale);
@@ -312,10 +307,10 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(const int* __restric
   const int64_t r0 = ((int64_t)blockIdx.x - rblocks) * zrows;
   const int nr = (int)min((int64_t)zrows, (int64_t)rows - r0);
   for (int k = threadIdx.x; k < kZeroRowsMax / 32; k += kBlock) seen[k] = 0;
-  const int64_t lo = block_lower_bound(K, n, (int)r0), hi = block_lower_bound(K, n, (int)(r0 + nr));
+  const int64_t lo = block_lower_bound(KP, n, (int)r0), hi = block_lower_bound(KP, n, (int)(r0 + nr));
   __syncthreads();
   for (int64_t i = lo + threadIdx.x; i < hi; i += kBlock) {
-    const int r = K[i] - (int)r0;
+    const int r = KP[i].x - (int)r0;
     atomicOr(&seen[r >> 5], 1u << (r & 31));
   }
   __syncthreads();
@@ -328,7 +323,7 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(const int* __restric
 // A chunk whose last token begins in it and goes on behind it joins that token's partial rows, in the chunks' order. Up to
 // kShort following chunks: the chunk's lane group alone; more: the whole block, its groups taking every GPB-th chunk.
 template <class T, int LPR, bool FULL>
-__global__ __launch_bounds__(kBlock) void embed_join_kernel(const int* __restrict__ K, int64_t n, int rows, int d,
+__global__ __launch_bounds__(kBlock) void embed_join_kernel(const int2* __restrict__ KP, int64_t n, int rows, int d,
                                                             float scale, T* __restrict__ gW,
                                                             const float* __restrict__ part, int chunk, int64_t chunks,
                                                             int ctiles) {
@@ -347,15 +342,15 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(const int* __restric
   int cur = rows;
   if (w < chunks - 1) {
     const int64_t a = w * chunk, b = a + chunk;
-    cur = K[b - 1];
-    mine = cur < rows && K[b] == cur && (K[a] != cur || a == 0 || K[a - 1] != cur);
+    cur = KP[b - 1].x;
+    mine = cur < rows && KP[b].x == cur && (KP[a].x != cur || a == 0 || KP[a - 1].x != cur);
   }
   // number of following chunks that begin with the token
   int64_t m = 0;
   bool more = mine;
   while (__any(more)) {
     const int64_t c = w + 1 + m + lig;
-    const bool hit = more && c < chunks && K[c * chunk] == cur;
+    const bool hit = more && c < chunks && KP[c * chunk].x == cur;
     const uint64_t bal = __ballot(hit) >> ((threadIdx.x & 63) / LPR * LPR);
     const uint64_t miss = LPR == 64 ? ~bal : (~bal & ((1ull << (LPR & 63)) - 1));
     const int run = miss ? __ffsll((unsigned long long)miss) - 1 : LPR;
@@ -388,7 +383,7 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(const int* __restric
       F sum = load_part<N, F, FULL>(part + (chunks + lw) * d + col, left);
 #pragma unroll
       for (int k = 0; k < GPB; ++k) sum += red[k * LPR + lig];
-      store_f32<T, FULL>(gW + (int64_t)K[lw * chunk + chunk - 1] * d + col, left, sum * scale);
+      store_f32<T, FULL>(gW + (int64_t)KP[lw * chunk + chunk - 1].x * d + col, left, sum * scale);
     }
     __syncthreads();
   }
@@ -403,7 +398,7 @@ struct Plan {
   int64_t per, blocks;       // radix: places of a block (whole tiles), blocks
   int chunk;
   int64_t chunks;
-  int64_t npad;              // K / P entries, whole batches
+  int64_t npad;              // (key, place) pairs, whole batches
   size_t bytes, off_hist, off_part;
 };
 
@@ -429,43 +424,36 @@ Plan plan_for(int64_t rows, int d, int64_t n) {
 }
 
 template <class I>
-int sort_places(const I* idx, int64_t n, IdxRule q, const Plan& p, char* ws, const int** Kout, const int** Pout,
-                hipStream_t s) {
-  int* A = reinterpret_cast<int*>(ws);
-  int* K[2] = {A, A + 2 * p.npad};
-  int* P[2] = {A + p.npad, A + 3 * p.npad};
-  *Kout = K[0];
-  *Pout = P[0];
+int sort_places(const I* idx, int64_t n, IdxRule q, const Plan& p, char* ws, const int2** sorted, hipStream_t s) {
+  int2* KP[2] = {reinterpret_cast<int2*>(ws), reinterpret_cast<int2*>(ws) + p.npad};
+  *sorted = KP[0];
   if (n == 0) return 0;
   if (p.ranked) {
-    hipLaunchKernelGGL(embed_rank_kernel<I>, dim3((unsigned)((n + 63) / 64)), dim3(kSortThreads), 0, s, idx, (int)n, q, K[0],
-                       P[0]);
+    hipLaunchKernelGGL(embed_rank_kernel<I>, dim3((unsigned)((n + 63) / 64)), dim3(kSortThreads), 0, s, idx, (int)n, q, KP[0]);
     MMSSL_LAUNCH_CHECK();
     return 0;
   }
   int* H = reinterpret_cast<int*>(ws + p.off_hist);
-  const int* Kin = nullptr;
-  const int* Pin = nullptr;
+  const int2* in = nullptr;
   const int mask = (1 << p.bits) - 1;
   for (int k = 0; k < p.passes; ++k) {
     const dim3 grid((unsigned)p.blocks), block(kSortThreads);
-    hipLaunchKernelGGL(embed_hist_kernel<I>, grid, block, 0, s, idx, Kin, n, q, p.per, k * p.bits, mask, H);
+    hipLaunchKernelGGL(embed_hist_kernel<I>, grid, block, 0, s, idx, in, n, q, p.per, k * p.bits, mask, H);
     MMSSL_LAUNCH_CHECK();
     if (p.per % (4 * kSortThreads) == 0)
-      hipLaunchKernelGGL((embed_scatter_kernel<I, 4>), grid, block, 0, s, idx, Kin, Pin, n, q, p.per, k * p.bits, mask, H,
-                         K[k & 1], P[k & 1]);
+      hipLaunchKernelGGL((embed_scatter_kernel<I, 4>), grid, block, 0, s, idx, in, n, q, p.per, k * p.bits, mask, H,
+                         KP[k & 1]);
     else
-      hipLaunchKernelGGL((embed_scatter_kernel<I, 1>), grid, block, 0, s, idx, Kin, Pin, n, q, p.per, k * p.bits, mask, H,
-                         K[k & 1], P[k & 1]);
+      hipLaunchKernelGGL((embed_scatter_kernel<I, 1>), grid, block, 0, s, idx, in, n, q, p.per, k * p.bits, mask, H,
+                         KP[k & 1]);
     MMSSL_LAUNCH_CHECK();
-    Kin = *Kout = K[k & 1];
-    Pin = *Pout = P[k & 1];
+    in = *sorted = KP[k & 1];
   }
   return 0;
 }
 
 template <class T, int LPR, bool FULL>
-int grad_launch(const int* K, const int* P, int64_t n, int rows, int d, const T* g, int64_t ldg, float scale, T* gW,
+int grad_launch(const int2* KP, int64_t n, int rows, int d, const T* g, int64_t ldg, float scale, T* gW,
                 float* part, const Plan& p, hipStream_t s) {
   const int vecs = (d + Vec<T>::N - 1) / Vec<T>::N;
   const int ctiles = (vecs + LPR - 1) / LPR;
@@ -475,11 +463,11 @@ int grad_launch(const int* K, const int* P, int64_t n, int rows, int d, const T*
   const int64_t zblocks = ((int64_t)rows + zrows - 1) / zrows;
   if (rblocks + zblocks > 0x7fffffff) return MMSSL_E_UNSUPP;
   if (rblocks + zblocks == 0) return 0;
-  hipLaunchKernelGGL((embed_grad_kernel<T, LPR, FULL>), dim3((unsigned)(rblocks + zblocks)), dim3(kBlock), 0, s, K, P, n, rows, d,
+  hipLaunchKernelGGL((embed_grad_kernel<T, LPR, FULL>), dim3((unsigned)(rblocks + zblocks)), dim3(kBlock), 0, s, KP, n, rows, d,
                      g, ldg, scale, gW, part, p.chunk, p.chunks, ctiles, rblocks, zrows);
   MMSSL_LAUNCH_CHECK();
   if (p.chunks > 1) {
-    hipLaunchKernelGGL((embed_join_kernel<T, LPR, FULL>), dim3((unsigned)rblocks), dim3(kBlock), 0, s, K, n, rows, d, scale, gW,
+    hipLaunchKernelGGL((embed_join_kernel<T, LPR, FULL>), dim3((unsigned)rblocks), dim3(kBlock), 0, s, KP, n, rows, d, scale, gW,
                        (const float*)part, p.chunk, p.chunks, ctiles);
     MMSSL_LAUNCH_CHECK();
   }
@@ -548,16 +536,16 @@ extern "C" int mmssl_embed_rows_bwd(const void* g, int64_t ldg, int dtype, const
   const IdxRule q{(int)rows, has_padding ? 1 : 0, padding_idx};
   const hipStream_t s = as_stream(stream);
   char* ws = static_cast<char*>(workspace);
-  const int *K = nullptr, *P = nullptr;
-  const int rc = idx_bytes == 8 ? sort_places((const int64_t*)idx, n, q, p, ws, &K, &P, s)
-                                : sort_places((const int32_t*)idx, n, q, p, ws, &K, &P, s);
+  const int2* KP = nullptr;
+  const int rc = idx_bytes == 8 ? sort_places((const int64_t*)idx, n, q, p, ws, &KP, s)
+                                : sort_places((const int32_t*)idx, n, q, p, ws, &KP, s);
   if (rc) return rc;
   float* part = reinterpret_cast<float*>(ws + p.off_part);
   const int lpr = lanes_for((d + (int)(16 / es) - 1) / (int)(16 / es));
 #define EMBED_GRAD_L(T, L)                                                                                              \
   return d % Vec<T>::N == 0                                                                                              \
-             ? grad_launch<T, L, true>(K, P, n, (int)rows, d, (const T*)g, ldg, scale, (T*)grad, part, p, s)             \
-             : grad_launch<T, L, false>(K, P, n, (int)rows, d, (const T*)g, ldg, scale, (T*)grad, part, p, s)
+             ? grad_launch<T, L, true>(KP, n, (int)rows, d, (const T*)g, ldg, scale, (T*)grad, part, p, s)             \
+             : grad_launch<T, L, false>(KP, n, (int)rows, d, (const T*)g, ldg, scale, (T*)grad, part, p, s)
 #define EMBED_GRAD(T)               \
   switch (lpr) {                    \
     case 8: EMBED_GRAD_L(T, 8);     \

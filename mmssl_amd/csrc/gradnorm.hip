@@ -2,8 +2,10 @@
 //
 //   n = sqrt(sum over all tensors of |g|^2);   out = g * c,  c = min(1, max_norm / (n + eps))
 //
-// A launch takes up to MMSSL_CLIP_MAX_TENSORS tensors of any of the three types and any size as kernel arguments (nothing is
-// uploaded, a captured graph replays them); its blocks share the tensors' chunks evenly and leave one partial sum each. The
+// Up to MMSSL_CLIP_MAX_TENSORS tensors of any of the three types and any size are kernel arguments; longer lists are written by
+// kernel arguments into a table in the workspace first, so that the norm and the scaling stay one launch each (600 tensors,
+// 60 M bf16: 150 us as seven launches each). Nothing is uploaded from host memory, a captured graph replays the list. The
+// blocks share the tensors' chunks evenly and leave one partial sum each. The
 // sums are in 64 bits: the square of every fp32 number is representable, nothing overflows or vanishes on the way, and the
 // conversions hide behind the loads. The scaling launch adds the partial sums up again in every block (a few KB out of the
 // cache) instead of waiting for a launch that would do it once, and walks the chunks from the back, where the norm's launch
@@ -36,16 +38,90 @@ struct NormList {                         // the same without outputs: half the 
   int32_t count;
 };
 
-template <class L>
-__device__ __forceinline__ int tensor_of(const L& l, int chunk) {
-  int lo = 0, hi = l.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (l.first[mid] <= chunk) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+// one tensor of a list in the workspace
+struct __attribute__((aligned(16))) Entry {
+  const void* g;
+  void* o;
+  int64_t n;
+  int32_t first;
+  int32_t dt;
+};
+
+__global__ __launch_bounds__(128) void table_kernel(List l, int32_t from, Entry* __restrict__ table) {
+  for (int i = threadIdx.x; i < l.count; i += 128) table[i] = {l.g[i], l.o[i], l.n[i], from + l.first[i], l.dt[i]};
 }
+
+// Where a chunk is: its tensor's type, first element of the chunk, elements from there on.
+struct Place {
+  const char* g;
+  char* o;
+  int64_t left;
+  int dt;
+};
+__device__ __forceinline__ Place place_of(const void* g, void* o, int64_t n, int dt, int chunk) {
+  const int64_t at = (int64_t)chunk * kChunk, size = dt == MMSSL_F32 ? 4 : 2;
+  return {static_cast<const char*>(g) + at * size, static_cast<char*>(o) + at * size, n - at, dt};
+}
+__device__ __forceinline__ void* out_of(const List& l, int t) { return l.o[t]; }
+__device__ __forceinline__ void* out_of(const NormList&, int) { return nullptr; }
+
+// Lists in the arguments: a search through scalar registers for each chunk, the chunks dealt to the blocks in turn.
+template <class L>
+struct Walk {
+  const L& l;
+  __device__ __forceinline__ Walk(const L& list) : l(list) {}
+  __device__ __forceinline__ int begin(int) const { return blockIdx.x; }
+  __device__ __forceinline__ int end(int chunks) const { return chunks; }
+  __device__ __forceinline__ int step() const { return gridDim.x; }
+  __device__ __forceinline__ int from_back(int i, int chunks) const { return chunks - 1 - i; }
+  __device__ __forceinline__ Place find(int chunk) const {
+    int lo = 0, hi = l.count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (l.first[mid] <= chunk) lo = mid;
+      else hi = mid - 1;
+    }
+    return place_of(l.g[lo], out_of(l, lo), l.n[lo], l.dt[lo], chunk - l.first[lo]);
+  }
+};
+
+// Lists in the workspace: a block's chunks follow each other; one search for the first by all threads at once (entries
+// counted whose first chunk is not behind it), then the entry stays in registers until its chunks end.
+struct Table {
+  const Entry* e;
+  int32_t count, chunks;
+};
+template <>
+struct Walk<Table> {
+  const Table l;
+  int at = -1, until = -1;                // the entry at hand, the chunk behind its last
+  Entry cur;
+  __device__ __forceinline__ Walk(const Table& table) : l(table) {}
+  __device__ __forceinline__ int begin(int chunks) const { return (int)((int64_t)chunks * blockIdx.x / gridDim.x); }
+  __device__ __forceinline__ int end(int chunks) const { return (int)((int64_t)chunks * (blockIdx.x + 1) / gridDim.x); }
+  __device__ __forceinline__ int step() const { return 1; }
+  __device__ __forceinline__ int from_back(int i, int) const { return i; }
+  __device__ __forceinline__ Place find(int chunk) {
+    if (chunk >= until) {
+      if (at < 0) {
+        int n = 0;
+        for (int i = 0; i < l.count; i += kBlock) {              // every thread of the block takes part
+          const int k = i + (int)threadIdx.x;
+          n += __syncthreads_count(k < l.count && l.e[k].first <= chunk);
+        }
+        at = n - 1;
+      } else {
+        while (at + 1 < l.count && l.e[at + 1].first <= chunk) ++at;
+      }
+      cur = l.e[at];
+      until = cur.first + (int)((cur.n + kChunk - 1) / kChunk);
+    }
+    return place_of(cur.g, cur.o, cur.n, cur.dt, chunk - cur.first);
+  }
+};
+template <class L>
+__device__ __forceinline__ int chunks_in(const L& l) { return l.first[l.count]; }
+__device__ __forceinline__ int chunks_in(const Table& l) { return l.chunks; }
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -60,41 +136,56 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// The elements of a chunk, `left` of them: all vectors are asked for before the first is used, also those of a tensor's last,
+// shorter chunk (with a loop there, lists of many small tensors waited once per 4 KB).
 template <class T>
-__device__ __forceinline__ double squares(const T* __restrict__ p, int left) {
-  constexpr int N = Vec<T>::N, IT = kChunk / (kBlock * N);
-  double a = 0.0;
-  if (left >= kChunk) {
-    typename Vec<T>::raw v[IT];
-#pragma unroll
-    for (int k = 0; k < IT; ++k) v[k] = load_raw<T, true>(p + (k * kBlock + threadIdx.x) * N, N);
+struct Chunk {
+  static constexpr int N = Vec<T>::N, IT = kChunk / (kBlock * N);
+  typedef typename Vec<T>::raw R;
+  R v[IT];
+  T last;                                 // one of the elements behind the last whole vector
+  int whole;
+  bool has_last;
+  __device__ __forceinline__ void load(const T* p, int left) {
+    whole = left / N * N;
+    has_last = whole + (int)threadIdx.x < left;
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      const typename Vec<T>::f32 f = to_f32<T>(v[k]);
-#pragma unroll
-      for (int e = 0; e < N; ++e) a = fma((double)f[e], (double)f[e], a);
+      const int i = (k * kBlock + threadIdx.x) * N;
+      v[k] = (R)(T)0.0f;
+      if (i < whole) v[k] = *reinterpret_cast<const R*>(p + i);
     }
-  } else {
-    for (int i = threadIdx.x * N; i < left; i += kBlock * N) {
-      const typename Vec<T>::f32 f = to_f32<T>(load_raw<T>(p + i, left - i));
-#pragma unroll
-      for (int e = 0; e < N; ++e) a = fma((double)f[e], (double)f[e], a);
-    }
+    last = (T)0.0f;
+    if (has_last) last = p[whole + threadIdx.x];
   }
-  return a;
+};
+
+template <class T>
+__device__ __forceinline__ double squares(const T* __restrict__ p, int left) {
+  Chunk<T> q;
+  q.load(p, left);
+  double a = 0.0;
+#pragma unroll
+  for (int k = 0; k < Chunk<T>::IT; ++k) {
+    const typename Vec<T>::f32 f = to_f32<T>(q.v[k]);
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; ++e) a = fma((double)f[e], (double)f[e], a);
+  }
+  return fma((double)(float)q.last, (double)(float)q.last, a);
 }
 
-__global__ __launch_bounds__(kBlock) void norm_kernel(NormList l, double* __restrict__ part) {
+template <class L>
+__global__ __launch_bounds__(kBlock) void norm_kernel(L l, double* __restrict__ part) {
   __shared__ double red[4];
-  const int chunks = l.first[l.count];
+  const int chunks = chunks_in(l);
+  Walk<L> w(l);
   double a = 0.0;
-  for (int ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
-    const int t = tensor_of(l, ch);
-    const int64_t at = (int64_t)(ch - l.first[t]) * kChunk;
-    const int left = (int)min((int64_t)kChunk, l.n[t] - at);
-    if (l.dt[t] == MMSSL_F32) a += squares(static_cast<const float*>(l.g[t]) + at, left);
-    else if (l.dt[t] == MMSSL_BF16) a += squares(static_cast<const bf16_t*>(l.g[t]) + at, left);
-    else a += squares(static_cast<const f16_t*>(l.g[t]) + at, left);
+  for (int ch = w.begin(chunks); ch < w.end(chunks); ch += w.step()) {
+    const Place p = w.find(ch);
+    const int left = (int)min((int64_t)kChunk, p.left);
+    if (p.dt == MMSSL_F32) a += squares(reinterpret_cast<const float*>(p.g), left);
+    else if (p.dt == MMSSL_BF16) a += squares(reinterpret_cast<const bf16_t*>(p.g), left);
+    else a += squares(reinterpret_cast<const f16_t*>(p.g), left);
   }
   a = block_sum(a, red);
   if (threadIdx.x == 0) part[blockIdx.x] = a;
@@ -115,52 +206,44 @@ __global__ __launch_bounds__(kBlock) void norm_finish_kernel(const double* __res
 
 template <class T>
 __device__ __forceinline__ void scaled(const T* p, T* o, int left, float c) {
-  constexpr int N = Vec<T>::N, IT = kChunk / (kBlock * N);
-  if (left >= kChunk) {
-    typename Vec<T>::raw v[IT];
+  Chunk<T> q;
+  q.load(p, left);
 #pragma unroll
-    for (int k = 0; k < IT; ++k)
-      v[k] = *reinterpret_cast<const typename Vec<T>::raw*>(p + (k * kBlock + threadIdx.x) * N);
-#pragma unroll
-    for (int k = 0; k < IT; ++k)
-      *reinterpret_cast<typename Vec<T>::raw*>(o + (k * kBlock + threadIdx.x) * N) =
-          __builtin_convertvector(to_f32<T>(v[k]) * c, typename Vec<T>::raw);
-  } else {
-    const int whole = left / N * N;
-    for (int i = threadIdx.x * N; i < whole; i += kBlock * N) {
-      const typename Vec<T>::raw v = *reinterpret_cast<const typename Vec<T>::raw*>(p + i);
-      *reinterpret_cast<typename Vec<T>::raw*>(o + i) = __builtin_convertvector(to_f32<T>(v) * c, typename Vec<T>::raw);
-    }
-    if (whole + (int)threadIdx.x < left) o[whole + threadIdx.x] = (T)((float)p[whole + threadIdx.x] * c);
+  for (int k = 0; k < Chunk<T>::IT; ++k) {
+    const int i = (k * kBlock + threadIdx.x) * Vec<T>::N;
+    if (i < q.whole)
+      *reinterpret_cast<typename Vec<T>::raw*>(o + i) =
+          __builtin_convertvector(to_f32<T>(q.v[k]) * c, typename Vec<T>::raw);
   }
+  if (q.has_last) o[q.whole + threadIdx.x] = (T)((float)q.last * c);
 }
 
 // `out` may be the gradients themselves: every element is read and written by one thread
-__global__ __launch_bounds__(kBlock) void clip_kernel(List l, const double* __restrict__ part, int nparts, float max_norm,
+template <class L>
+__global__ __launch_bounds__(kBlock) void clip_kernel(L l, const double* __restrict__ part, int nparts, float max_norm,
                                                       float eps, int same, float* __restrict__ norm) {
   __shared__ double red[4];
   const double n = norm_of(part, nparts, red);
   const double q = (double)max_norm / (n + (double)eps);
   const float c = q >= 1.0 ? 1.0f : (float)q;            // a NaN stays one
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)n;
+  if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)n;
   if (same && c == 1.0f) return;                         // in place, below the largest norm: times 1
-  const int chunks = l.first[l.count];
-  for (int ch = chunks - 1 - (int)blockIdx.x; ch >= 0; ch -= gridDim.x) {
-    const int t = tensor_of(l, ch);
-    const int64_t at = (int64_t)(ch - l.first[t]) * kChunk;
-    const int left = (int)min((int64_t)kChunk, l.n[t] - at);
-    if (l.dt[t] == MMSSL_F32) scaled(static_cast<const float*>(l.g[t]) + at, static_cast<float*>(l.o[t]) + at, left, c);
-    else if (l.dt[t] == MMSSL_BF16)
-      scaled(static_cast<const bf16_t*>(l.g[t]) + at, static_cast<bf16_t*>(l.o[t]) + at, left, c);
-    else scaled(static_cast<const f16_t*>(l.g[t]) + at, static_cast<f16_t*>(l.o[t]) + at, left, c);
+  const int chunks = chunks_in(l);
+  Walk<L> w(l);
+  for (int i = w.begin(chunks); i < w.end(chunks); i += w.step()) {
+    const Place p = w.find(w.from_back(i, chunks));
+    const int left = (int)min((int64_t)kChunk, p.left);
+    if (p.dt == MMSSL_F32) scaled(reinterpret_cast<const float*>(p.g), reinterpret_cast<float*>(p.o), left, c);
+    else if (p.dt == MMSSL_BF16) scaled(reinterpret_cast<const bf16_t*>(p.g), reinterpret_cast<bf16_t*>(p.o), left, c);
+    else scaled(reinterpret_cast<const f16_t*>(p.g), reinterpret_cast<f16_t*>(p.o), left, c);
   }
 }
 
 int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
-// the tensors [a, b) of one launch; 0, or the error
+// the tensors [a, b) as kernel arguments
 template <class L>
-int fill(L& l, const void* const* grads, const int64_t* numel, const int32_t* dtypes, int a, int b) {
+void fill(L& l, const void* const* grads, const int64_t* numel, const int32_t* dtypes, int a, int b) {
   int64_t chunks = 0;
   l.count = b - a;
   for (int i = a; i < b; ++i) {
@@ -169,10 +252,8 @@ int fill(L& l, const void* const* grads, const int64_t* numel, const int32_t* dt
     l.dt[i - a] = (uint8_t)dtypes[i];
     l.first[i - a] = (int32_t)chunks;
     chunks += chunks_of(numel[i]);
-    if (chunks > 0x3fffffff) return MMSSL_E_UNSUPP;
   }
   l.first[b - a] = (int32_t)chunks;
-  return 0;
 }
 
 int check_list(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int count) {
@@ -181,45 +262,78 @@ int check_list(const void* const* grads, const int64_t* numel, const int32_t* dt
     if (numel[i] < 0 || !known_dtype(dtypes[i])) return MMSSL_E_BADARG;
     if (numel[i] > 0 && (!grads[i] || !aligned_to(grads[i], dtype_bytes(dtypes[i])))) return MMSSL_E_BADARG;
   }
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (numel[i] > (int64_t)0x3fffffff * kChunk) return MMSSL_E_UNSUPP;
+    chunks += chunks_of(numel[i]);
+    if (chunks > 0x3fffffff) return MMSSL_E_UNSUPP;
+  }
   return 0;
 }
 
-int launches_of(int count) { return (count + kMaxT - 1) / kMaxT; }
+// workspace: the blocks' sums, then the table of a long list
+constexpr size_t kPartBytes = (size_t)kMaxBlocks * 8;
+size_t ws_bytes(int count) { return kPartBytes + (count > kMaxT ? (size_t)count * sizeof(Entry) : 0); }
 
-// partial sums of all launches; blocks of launch k in *blocks (NULL: not wanted)
-int norm_launches(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int count, double* part,
-                  hipStream_t s, int* nparts) {
-  int used = 0;
+int total_chunks(const int64_t* numel, int count) {
+  int64_t c = 0;
+  for (int i = 0; i < count; ++i) c += chunks_of(numel[i]);
+  return (int)c;                          // check_list has seen it
+}
+
+// the long list's table; `outs` may be NULL
+int write_table(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, int count,
+                Entry* table, hipStream_t s) {
+  int32_t from = 0;
   for (int a = 0; a < count; a += kMaxT) {
     const int b = std::min(count, a + kMaxT);
-    NormList l;
-    if (int rc = fill(l, grads, numel, dtypes, a, b)) return rc;
-    const int blocks = std::min(l.first[l.count], kMaxBlocks);
-    if (blocks == 0) continue;
-    hipLaunchKernelGGL(norm_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, s, l, part + used);
+    List l;
+    fill(l, grads, numel, dtypes, a, b);
+    for (int i = a; i < b; ++i) l.o[i - a] = outs ? outs[i] : nullptr;
+    hipLaunchKernelGGL(table_kernel, dim3(1), dim3(128), 0, s, l, from, table + a);
     MMSSL_LAUNCH_CHECK();
-    used += blocks;
+    from += l.first[l.count];
   }
-  *nparts = used;
   return 0;
+}
+
+template <class L>
+int norm_launch(const L& l, int blocks, double* part, hipStream_t s) {
+  hipLaunchKernelGGL(norm_kernel<L>, dim3((unsigned)blocks), dim3(kBlock), 0, s, l, part);
+  MMSSL_LAUNCH_CHECK();
+  return 0;
+}
+
+// grads -> the blocks' sums in `part`; a long list's table is written on the way
+int sums_of(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, int count, int chunks,
+            void* workspace, hipStream_t s) {
+  double* part = static_cast<double*>(workspace);
+  const int blocks = std::min(chunks, kMaxBlocks);
+  if (count > kMaxT) {
+    Entry* table = reinterpret_cast<Entry*>(static_cast<char*>(workspace) + kPartBytes);
+    if (int rc = write_table(grads, outs, numel, dtypes, count, table, s)) return rc;
+    return norm_launch(Table{table, count, chunks}, blocks, part, s);
+  }
+  NormList l;
+  fill(l, grads, numel, dtypes, 0, count);
+  return norm_launch(l, blocks, part, s);
 }
 
 }  // namespace
 
-extern "C" size_t mmssl_grad_norm_workspace_bytes(int count) {
-  return count < 0 ? 0 : (size_t)launches_of(count) * kMaxBlocks * 8 + 16;
-}
+extern "C" size_t mmssl_grad_norm_workspace_bytes(int count) { return count < 0 ? 0 : ws_bytes(count); }
 
 extern "C" int mmssl_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int count, float* norm,
                                void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_list(grads, numel, dtypes, count)) return rc;
   if (!norm) return MMSSL_E_BADARG;
-  if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < mmssl_grad_norm_workspace_bytes(count))
-    return MMSSL_E_WORKSPACE;
-  double* part = static_cast<double*>(workspace);
-  int nparts = 0;
-  if (int rc = norm_launches(grads, numel, dtypes, count, part, as_stream(stream), &nparts)) return rc;
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kBlock), 0, as_stream(stream), (const double*)part, nparts, norm);
+  if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < ws_bytes(count)) return MMSSL_E_WORKSPACE;
+  const hipStream_t s = as_stream(stream);
+  const int chunks = total_chunks(numel, count);
+  if (chunks)
+    if (int rc = sums_of(grads, nullptr, numel, dtypes, count, chunks, workspace, s)) return rc;
+  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kBlock), 0, s, static_cast<const double*>(workspace),
+                     std::min(chunks, kMaxBlocks), norm);
   MMSSL_LAUNCH_CHECK();
   return 0;
 }
@@ -229,35 +343,32 @@ extern "C" int mmssl_clip_grads(const void* const* grads, void* const* outs, con
                                 void* stream) {
   if (int rc = check_list(grads, numel, dtypes, count)) return rc;
   if (!norm || !(max_norm >= 0.f) || !(eps >= 0.f) || (count > 0 && !outs)) return MMSSL_E_BADARG;
-  for (int i = 0; i < count; ++i)
+  int same = 1;
+  for (int i = 0; i < count; ++i) {
     if (numel[i] > 0 && (!outs[i] || !aligned_to(outs[i], dtype_bytes(dtypes[i])))) return MMSSL_E_BADARG;
-  if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < mmssl_grad_norm_workspace_bytes(count))
-    return MMSSL_E_WORKSPACE;
-  double* part = static_cast<double*>(workspace);
+    same &= numel[i] == 0 || outs[i] == grads[i];
+  }
+  if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < ws_bytes(count)) return MMSSL_E_WORKSPACE;
   const hipStream_t s = as_stream(stream);
-  int nparts = 0;
-  if (int rc = norm_launches(grads, numel, dtypes, count, part, s, &nparts)) return rc;
-  if (nparts == 0) {
-    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kBlock), 0, s, (const double*)part, 0, norm);
+  const int chunks = total_chunks(numel, count), blocks = std::min(chunks, kMaxBlocks);
+  const double* part = static_cast<const double*>(workspace);
+  if (chunks == 0) {
+    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kBlock), 0, s, part, 0, norm);
     MMSSL_LAUNCH_CHECK();
     return 0;
   }
-  bool told = false;
-  for (int b = count; b > 0; b = (b - 1) / kMaxT * kMaxT) {            // the last tensors first: they were read last
-    const int a = (b - 1) / kMaxT * kMaxT;
+  if (int rc = sums_of(grads, outs, numel, dtypes, count, chunks, workspace, s)) return rc;
+  if (count > kMaxT) {
+    const Table l{reinterpret_cast<const Entry*>(static_cast<const char*>(workspace) + kPartBytes), count, chunks};
+    hipLaunchKernelGGL(clip_kernel<Table>, dim3((unsigned)blocks), dim3(kBlock), 0, s, l, part, blocks, max_norm, eps, same,
+                       norm);
+  } else {
     List l;
-    if (int rc = fill(l, grads, numel, dtypes, a, b)) return rc;
-    int same = 1;
-    for (int i = a; i < b; ++i) {
-      l.o[i - a] = outs[i];
-      same &= numel[i] == 0 || outs[i] == grads[i];
-    }
-    const int blocks = std::min(l.first[l.count], kMaxBlocks);
-    if (blocks == 0) continue;
-    hipLaunchKernelGGL(clip_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, s, l, (const double*)part, nparts, max_norm, eps,
-                       same, told ? (float*)nullptr : norm);
-    MMSSL_LAUNCH_CHECK();
-    told = true;
+    fill(l, grads, numel, dtypes, 0, count);
+    for (int i = 0; i < count; ++i) l.o[i] = outs[i];
+    hipLaunchKernelGGL(clip_kernel<List>, dim3((unsigned)blocks), dim3(kBlock), 0, s, l, part, blocks, max_norm, eps, same,
+                       norm);
   }
+  MMSSL_LAUNCH_CHECK();
   return 0;
 }

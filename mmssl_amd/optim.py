@@ -194,7 +194,7 @@ def _grads(grads):
 
 def grad_norm(grads):
     """The 2-norm of all elements of a list of gradients together (fp32 / bf16 / fp16, mixed, any sizes) as a 0-dim fp32 device
-    tensor: one launch per 96 tensors and a small one, 64-bit sums in a fixed order, nothing read back."""
+    tensor: one launch over all of them and a small one, 64-bit sums in a fixed order, nothing read back."""
     return _lib.binding().grad_norm(_grads(grads))
 
 
