@@ -19,8 +19,10 @@ using namespace mmssl;
 namespace {
 
 constexpr int kMaxT = MMSSL_CLIP_MAX_TENSORS;
-constexpr int kChunk = 8192;              // elements of a chunk
-constexpr int kMaxBlocks = 1024;          // of one launch
+// Elements of a chunk, blocks of a launch: 384 M fp32 in 9 tensors 864 us (8192 and 1024: 868; 16384: 881), 600 tensors of 60 M
+// bf16 86 us (90; 93), 24 tensors of 0.3 M fp32 8.9 us (9.4; 11.1).
+constexpr int kChunk = 4096;
+constexpr int kMaxBlocks = 2048;
 
 struct List {
   const void* g[kMaxT];
@@ -137,7 +139,7 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 }
 
 // The elements of a chunk, `left` of them: all vectors are asked for before the first is used, also those of a tensor's last,
-// shorter chunk (with a loop there, lists of many small tensors waited once per 4 KB).
+// shorter chunk (with a loop there, lists of many small tensors waited once per 4 KB: 600 of 60 M bf16, norm alone 54 -> 42 us).
 template <class T>
 struct Chunk {
   static constexpr int N = Vec<T>::N, IT = kChunk / (kBlock * N);

@@ -190,7 +190,6 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
   __shared__ float red[3 * kWaves];
   __shared__ uint32_t bound[kWaves];
   __shared__ uint64_t pairs[TOP ? kCand : 1];
-  uint2* raws = reinterpret_cast<uint2*>(pairs);
   __shared__ int n_pairs;
   __shared__ int count[2 * kWaves];
   const int64_t row = blockIdx.x / splits;
@@ -299,7 +298,7 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
             if (h) {
               if (h >> lane & 1) {                                // value and column for now: few instructions a hit
                 const int at = i + __builtin_amdgcn_mbcnt_hi((uint32_t)(h >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)h, 0));
-                raws[at] = make_uint2(__float_as_uint((float)raw[v][e]), (v * kBlock + threadIdx.x) * N + e);
+                pairs[at] = ((uint64_t)__float_as_uint((float)raw[v][e]) << 32) | ((v * kBlock + threadIdx.x) * N + e);
               }
               i += __popcll(h);
             }
@@ -310,8 +309,8 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
     n = n_pairs;
     if (n <= kCand) {
       for (int j = threadIdx.x; j < n; j += kBlock) {             // an entry is its thread's alone
-        const uint2 q = raws[j];
-        pairs[j] = pair_of(__uint_as_float(q.x), c0 + q.y);
+        const uint64_t q = pairs[j];
+        pairs[j] = pair_of(__uint_as_float((uint32_t)(q >> 32)), c0 + (uint32_t)q);
       }
       __syncthreads();
     }

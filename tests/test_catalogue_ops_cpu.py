@@ -105,3 +105,15 @@ def test_c_entry_points_refuse_bad_arguments():
         args[at] = value
         assert L.mmssl_clip_grads(*args) == code, (at, value)
     assert L.mmssl_grad_norm_workspace_bytes(-1) == 0
+
+
+def test_missing_binding_fails_loudly():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ("import sys\nsys.modules['mmssl_amd._torch_binding'] = None\nimport torch\nfrom mmssl_amd import ops, _lib\n"
+            "try:\n    ops.layernorm_rows(torch.zeros(2, 4))\nexcept _lib.MmsslError as e:\n"
+            "    print('LOUD', 'no fallback' in str(e))\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert "LOUD True" in r.stdout, r.stdout + r.stderr

@@ -781,3 +781,114 @@ def test_catalogue_operators_on_two_streams_at_once():
     torch.cuda.synchronize()
     for o in got:
         assert all(torch.equal(a, b) for a, b in zip(o, want))
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+def test_catalogue_operators_refuse():
+    from mmssl_amd import ops, optim
+    from mmssl_amd._lib import MmsslError
+    x = torch.randn(6, 40, device=DEV)
+    idx = torch.zeros(6, dtype=torch.int64, device=DEV)
+    w = torch.ones(40, device=DEV)
+    half = x.half()
+    refused = [
+        lambda: ops.embed_rows(x.double(), idx), lambda: ops.embed_rows(x[0], idx), lambda: ops.embed_rows(x.t(), idx),
+        lambda: ops.embed_rows(x, idx.float()), lambda: ops.embed_rows(x, idx.bool()), lambda: ops.embed_rows([1.0], idx),
+        lambda: ops.embed_rows(x[:, :0], idx), lambda: ops.embed_rows(x.to_sparse(), idx),
+        lambda: ops.layernorm_rows(x.double()), lambda: ops.layernorm_rows(x.int()), lambda: ops.layernorm_rows(x[:, :0]),
+        lambda: ops.layernorm_rows(x, w[:39]), lambda: ops.layernorm_rows(x, w[None]), lambda: ops.layernorm_rows(x, w.half()),
+        lambda: ops.layernorm_rows(half, w, w.half()), lambda: ops.layernorm_rows(x, w.cpu()),
+        lambda: ops.layernorm_rows(x, eps=-1.0), lambda: ops.layernorm_rows(x, eps=float("nan")),
+        lambda: ops.layernorm_rows(x, eps=float("inf")), lambda: ops.layernorm_rows(torch.tensor(1.0, device=DEV)),
+        lambda: ops.logprobs_rows(x, idx, k=41), lambda: ops.logprobs_rows(x, idx, k=-1),
+        lambda: ops.logprobs_rows(torch.randn(6, 400, device=DEV), idx, k=129), lambda: ops.logprobs_rows(x, idx[:5]),
+        lambda: ops.logprobs_rows(x, idx[None]), lambda: ops.logprobs_rows(x, idx.float()),
+        lambda: ops.logprobs_rows(x, idx, temperature=0.0), lambda: ops.logprobs_rows(x, idx, temperature=-1.0),
+        lambda: ops.logprobs_rows(x, idx, temperature=float("nan")), lambda: ops.logprobs_rows(x, idx, temperature=float("inf")),
+        lambda: ops.logprobs_rows(x.double(), idx), lambda: ops.logprobs_rows(x[:, :0], idx),
+        lambda: optim.clip_grads([x], 1.0, out=[half]), lambda: optim.clip_grads([x], 1.0, out=[x[:5].clone()]),
+        lambda: optim.clip_grads([x, w], 1.0, out=[x]), lambda: optim.clip_grads([x, x.cpu()], 1.0),
+        lambda: optim.clip_grads([x, x], 1.0), lambda: optim.clip_grads([x[:4], x[2:]], 1.0),
+        lambda: optim.clip_grads([x[0], x[1]], 1.0, out=[x[1], x[2]]), lambda: optim.clip_grads([x.t()], 1.0),
+        lambda: optim.clip_grads([x.double()], 1.0), lambda: optim.clip_grads([x], float("nan")),
+        lambda: optim.grad_norm([x, x.cpu()]), lambda: optim.grad_norm([x.t()]), lambda: optim.grad_norm([]),
+    ]
+    before = x.clone()
+    for i, fn in enumerate(refused):
+        try:
+            fn()
+        except MmsslError:
+            continue
+        raise AssertionError("case %d was not refused" % i)
+    assert torch.equal(x, before)
+    # read-only lists may name a tensor twice, and an empty tensor is no overlap
+    assert abs(float(optim.grad_norm([x, x])) - 2 ** 0.5 * float(x.norm())) < 1e-4
+    e = torch.empty(0, device=DEV)
+    optim.clip_grads([e, x.clone(), e], 1.0)
+
+
+def test_gradients_are_not_differentiable_again():
+    from mmssl_amd import ops
+    x = torch.randn(6, 40, device=DEV, requires_grad=True)
+    idx = torch.zeros(6, dtype=torch.int64, device=DEV)
+    for out in (ops.embed_rows(x, idx), ops.layernorm_rows(x), ops.logprobs_rows(x, idx)[0]):
+        with pytest.raises(RuntimeError, match="not differentiable again"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+def test_modes_without_gradients_and_changed_inputs():
+    from mmssl_amd import ops, optim
+    x = torch.randn(6, 40, device=DEV, requires_grad=True)
+    idx = torch.arange(6, device=DEV)
+    want = ops.layernorm_rows(x).detach()
+    with torch.inference_mode():
+        got = ops.layernorm_rows(x)
+        assert torch.equal(got, want) and not got.requires_grad
+        g = torch.ones(5, device=DEV)
+        optim.clip_grads([g], 1.0)
+    with torch.no_grad():
+        assert not ops.embed_rows(x, idx).requires_grad and not ops.logprobs_rows(x, idx)[0].requires_grad
+    y = x * 1.0
+    out = ops.logprobs_rows(y, idx)[0]
+    optim.clip_grads([y.detach()], 0.5)                       # changes what the backward pass needs
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    # only some of the inputs want gradients
+    w = torch.ones(40, device=DEV, requires_grad=True)
+    b = torch.zeros(40, device=DEV)
+    a = x.detach()
+    (gw,) = torch.autograd.grad(ops.layernorm_rows(a, w, b).sum(), w)
+    assert torch.allclose(gw, torch.nn.functional.layer_norm(a, (40,)).sum(0), atol=1e-4)
+    b.requires_grad_(True)
+    (gb,) = torch.autograd.grad(ops.layernorm_rows(a, None, b).sum(), b)
+    assert torch.equal(gb, torch.full_like(gb, 6.0))
+    (gx,) = torch.autograd.grad(ops.layernorm_rows(x, w.detach(), b.detach()).sum(), x)
+    assert float(gx.abs().max()) < 1e-4                       # the rows' gradients of a plain sum cancel
+
+
+def test_long_gradient_lists_in_captured_graphs():
+    """Lists past the kernel arguments' go through a table in the workspace: two graphs with their own, replayed in turn with
+    eager calls between them."""
+    from mmssl_amd import optim
+    g0 = gen(81)
+    sizes = [int(v) for v in torch.randint(1, 20000, (250,), generator=g0)]
+    stream = torch.cuda.Stream()
+    graphs = []
+    for k in range(2):
+        grads = [torch.randn(n, generator=g0).to(TYPES[(i + k) % 3]).to(DEV) for i, n in enumerate(sizes)]
+        out = [torch.empty_like(g) for g in grads]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            norm = optim.clip_grads(grads, 2.0, out=out)
+        graphs.append((graph, grads, out, norm))
+    for turn in range(4):
+        for graph, grads, out, norm in graphs:
+            for g in grads:
+                g.mul_(0.5 if turn % 2 else 3.0)
+            graph.replay()
+            want = [torch.empty_like(g) for g in grads]
+            eager = optim.clip_grads(grads, 2.0, out=want)
+            torch.cuda.synchronize()
+            assert torch.equal(norm, eager)
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
