@@ -780,7 +780,8 @@ int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_t rows, int
                         float* top_logp, int64_t* top_idx, float* stats, void* workspace, size_t workspace_bytes,
                         void* stream);
 /* Its gradient GX [rows, cols] (contiguous, X's type) from the gradients of logp, entropy [rows] and top_logp [rows, k] (each
- * may be NULL: 0). Ignored and out-of-range targets name no column; a row of nothing but -inf gets zeros. */
+ * may be NULL: 0). The gradient of an ignored or out-of-range target's logp counts as 0; a row of nothing but -inf gets
+ * zeros. */
 int mmssl_logprobs_rows_bwd(const void* X, int64_t ldx, int dtype, int64_t rows, int64_t cols, const void* target,
                             int target_bytes, int64_t ignore_index, int k, float temperature, const int64_t* top_idx,
                             const float* stats, const float* glogp, const float* gentropy, const float* gtop, void* GX,

@@ -515,7 +515,8 @@ __global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X,
   const bool empty = st.y == __builtin_inff();
   const float m = empty ? 0.f : st.x, l2 = empty ? 0.f : st.y;
   const int64_t t = target64 ? target64[row] : (int64_t)target32[row];
-  const float gt = (glogp && t != ignore) ? glogp[row] : 0.f;
+  const bool asked = t != ignore && t >= 0 && t < cols;            // the target names a column
+  const float gt = glogp && asked ? glogp[row] : 0.f;
   float g = gt;
   if (gtop)
     for (int i = 0; i < k; ++i) g += gtop[row * k + i];
@@ -546,8 +547,8 @@ __global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X,
   const int named = 1 + (gtop ? k : 0);
   for (int i = threadIdx.x; i < named; i += kBlock) {
     const int64_t j = i ? top_idx[row * k + i - 1] : t;
-    if (j < c0 || j >= min(cols, c0 + LEN) || empty || (i == 0 && t == ignore)) continue;
-    if (i && j == t && t != ignore) continue;
+    if (j < c0 || j >= min(cols, c0 + LEN) || empty || (i == 0 && !asked)) continue;
+    if (i && j == t && asked) continue;
     float own = i ? gtop[row * k + i - 1] : gt;
     if (i == 0 && gtop)
       for (int h = 0; h < k; ++h)

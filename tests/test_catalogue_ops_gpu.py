@@ -331,9 +331,10 @@ def logprobs_exact(x, target, k, temperature, ignore, grads=None):
     outs = [held32(logp), h, held32(lp.gather(1, idx)), idx]
     if grads is not None:
         gl, gh, gt = (g.double() for g in grads)
-        gl = torch.where(target == ignore, torch.zeros_like(gl), gl)
+        asked = ok & (target != ignore)
+        gl = torch.where(asked, gl, torch.zeros_like(gl))
         named = torch.zeros_like(z)
-        named[row[ok & (target != ignore)], target[ok & (target != ignore)].long()] += gl[ok & (target != ignore)]
+        named[row[asked], target[asked].long()] += gl[asked]
         named.scatter_add_(1, idx, gt)
         gx = named - p * (gl + gt.sum(1))[:, None] - gh[:, None] * p * (held + h[:, None])
         gx[empty] = 0.0
