@@ -339,6 +339,52 @@ __global__ __launch_bounds__(kBlock) void lp_slice_kernel(const T* __restrict__ 
   }
 }
 
+// ---- forward: short rows without alternatives: a wave a row, no barriers (100 K rows of 1000 fp32: 150 us with a block a row) ---
+template <class T, int NV, bool FULL>
+__global__ __launch_bounds__(kBlock) void lp_short_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows, int cols, float c,
+                                                          float inv_t, RowOut o) {
+  constexpr int N = Vec<T>::N;
+  typedef typename Vec<T>::raw R;
+  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const T* x = X + row * ldx;
+  R raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int at = (v * 64 + lane) * N;
+    raw[v] = (R)(T)(-__builtin_inff());
+    if (FULL ? at < cols : at + N <= cols) {
+      raw[v] = load_raw<T, true>(x + at, N);
+    } else if (!FULL) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (at + e < cols) raw[v][e] = x[at + e];
+    }
+  }
+  const float at_target = lane == 0 ? target_score(x, cols, row, o) : 0.f;
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < N; ++e) m = fmaxf(m, (float)raw[v][e]);
+  m = group_max<64>(m);
+  const float base = m == -__builtin_inff() ? 0.f : m;
+  Sums z = {m, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float y = ((float)raw[v][e] - base) * c;
+      const float p = __builtin_amdgcn_exp2f(y);
+      z.s += p;
+      z.a = fmaf(p, fmaxf(y, kFar), z.a);
+    }
+  z.s = group_sum<64>(z.s);
+  z.a = group_sum<64>(z.a);
+  if (lane == 0) write_row(at_target, cols, row, stat_of(z), inv_t, o);
+}
+
 // ---- forward: the slices of a row -------------------------------------------------------------------------------------
 // These kernels run once through little data: what they cost is misses, of data and of instructions. What can be asked for at
 // once is, and their loops stay rolled (the same with 16 pairs a thread in unrolled registers: 20 us for one row of 1 M
@@ -491,24 +537,29 @@ __global__ __launch_bounds__(kBlock) void lp_join_top_kernel(const T* __restrict
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
-template <class T, int NV, bool FULL>
-__global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X, int64_t ldx, int64_t cols, int splits,
+// LANES of a block a slice: a block, or a wave (short rows: 100 K rows of 1000 bf16 127 us with a block a row)
+template <class T, int LANES, int NV, bool FULL>
+__global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows, int64_t cols,
+                                                        int splits,
                                                         float c, float inv_t, int k, const int64_t* __restrict__ target64,
                                                         const int32_t* __restrict__ target32, int64_t ignore,
                                                         const int64_t* __restrict__ top_idx,
                                                         const float4* __restrict__ stats, const float* __restrict__ glogp,
                                                         const float* __restrict__ gent, const float* __restrict__ gtop,
                                                         T* __restrict__ GX) {
-  constexpr int N = Vec<T>::N, LEN = kBlock * NV * N;
+  constexpr int N = Vec<T>::N, LEN = LANES * NV * N;
   typedef typename Vec<T>::f32 F;
-  const int64_t row = blockIdx.x / splits;
-  const int64_t c0 = (int64_t)(blockIdx.x % splits) * LEN;
+  const int tid = threadIdx.x & (LANES - 1);
+  const int64_t part = (int64_t)blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+  const bool there = part < rows * splits;         // the last block of short rows holds fewer
+  const int64_t row = there ? part / splits : 0;
+  const int64_t c0 = there ? part % splits * LEN : cols;
   const T* x = X + row * ldx;
   T* gx = GX + row * cols;
   typename Vec<T>::raw raw[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int64_t at = c0 + (v * kBlock + threadIdx.x) * N;
+    const int64_t at = c0 + (v * LANES + tid) * N;
     if (at < cols) raw[v] = load_raw<T, FULL>(x + at, (int)min((int64_t)N, cols - at));
   }
   const float4 st = stats[row];
@@ -531,7 +582,7 @@ __global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X,
   };
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int64_t at = c0 + (v * kBlock + threadIdx.x) * N;
+    const int64_t at = c0 + (v * LANES + tid) * N;
     if (at < cols) {
       const F f = to_f32<T>(raw[v]);
       F y;
@@ -545,7 +596,7 @@ __global__ __launch_bounds__(kBlock) void lp_bwd_kernel(const T* __restrict__ X,
   __threadfence_block();
   __syncthreads();
   const int named = 1 + (gtop ? k : 0);
-  for (int i = threadIdx.x; i < named; i += kBlock) {
+  for (int i = tid; i < named; i += LANES) {
     const int64_t j = i ? top_idx[row * k + i - 1] : t;
     if (j < c0 || j >= min(cols, c0 + LEN) || empty || (i == 0 && !asked)) continue;
     if (i && j == t && asked) continue;
@@ -580,6 +631,9 @@ Cut cut_for(int64_t rows, int64_t cols, int es) {
   return q;
 }
 
+// Rows that a wave takes alone (32 values a lane), where they are enough to fill the chip; fewer are cut into slices.
+bool short_rows(int64_t rows, int64_t cols) { return cols <= 2048 && rows >= 2048; }
+
 size_t ws_bytes(int64_t rows, const Cut& q, int k) {
   if (q.splits == 1) return 16;
   const size_t sums = ((size_t)rows * q.splits * sizeof(Sums) + 15) / 16 * 16;
@@ -612,17 +666,36 @@ extern "C" int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_
   if (!X || !target || !logp || !entropy || ldx < 0 || (k > 0 && (!top_logp || !top_idx))) return MMSSL_E_BADARG;
   if (!aligned_to(X, es) || !aligned_to(target, target_bytes) || !aligned_to(stats, 16) || !aligned_to(top_idx, 8))
     return MMSSL_E_BADARG;
-  const Cut q = cut_for(rows, cols, (int)es);
-  if (q.splits > 1 && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < ws_bytes(rows, q, k)))
-    return MMSSL_E_WORKSPACE;
   const float c = (float)((double)kLog2e / temperature), inv_t = (float)(1.0 / (double)temperature);
-  Sums* sums = static_cast<Sums*>(workspace);
-  uint64_t* cand = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) +
-                                               ((size_t)rows * q.splits * sizeof(Sums) + 15) / 16 * 16);
   RowOut o{target_bytes == 8 ? static_cast<const int64_t*>(target) : nullptr,
            target_bytes == 4 ? static_cast<const int32_t*>(target) : nullptr,
            ignore_index, logp, entropy, top_logp, top_idx, reinterpret_cast<float4*>(stats)};
   const hipStream_t s = as_stream(stream);
+  if (k == 0 && short_rows(rows, cols)) {
+    const dim3 grid((unsigned)((rows + kWaves - 1) / kWaves));
+#define LP_SHORT_F(T, V, F)                                                                                              \
+  hipLaunchKernelGGL((lp_short_kernel<T, V, F>), grid, dim3(kBlock), 0, s, (const T*)X, ldx, rows, (int)cols, c, inv_t, o)
+#define LP_SHORT_V(T, V)                            \
+  do {                                              \
+    if (cols % Vec<T>::N == 0) LP_SHORT_F(T, V, true); \
+    else LP_SHORT_F(T, V, false);                   \
+  } while (0)
+#define LP_SHORT(T)                                                       \
+  do {                                                                    \
+    if (cols <= 512) LP_SHORT_V(T, 8 / Vec<T>::N);                        \
+    else if (cols <= 1024) LP_SHORT_V(T, 16 / Vec<T>::N);                 \
+    else LP_SHORT_V(T, 32 / Vec<T>::N);                                   \
+  } while (0)
+    MMSSL_BY_DTYPE(dtype, LP_SHORT);
+    MMSSL_LAUNCH_CHECK();
+    return 0;
+  }
+  const Cut q = cut_for(rows, cols, (int)es);
+  if (q.splits > 1 && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < ws_bytes(rows, q, k)))
+    return MMSSL_E_WORKSPACE;
+  Sums* sums = static_cast<Sums*>(workspace);
+  uint64_t* cand = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) +
+                                               ((size_t)rows * q.splits * sizeof(Sums) + 15) / 16 * 16);
   const dim3 grid((unsigned)(rows * q.splits)), block(kBlock);
 #define LP_SLICE_T(T, V, F, TOP)                                                                                         \
   hipLaunchKernelGGL((lp_slice_kernel<T, V, F, TOP>), grid, block, 0, s, (const T*)X, ldx, cols, q.len, (int)q.splits, c, \
@@ -676,14 +749,21 @@ extern "C" int mmssl_logprobs_rows_bwd(const void* X, int64_t ldx, int dtype, in
   const int64_t* t64 = target_bytes == 8 ? static_cast<const int64_t*>(target) : nullptr;
   const int32_t* t32 = target_bytes == 4 ? static_cast<const int32_t*>(target) : nullptr;
   constexpr int NV = 4;
-#define LP_BWD_F(T, F)                                                                                                   \
-  hipLaunchKernelGGL((lp_bwd_kernel<T, NV, F>), dim3((unsigned)(rows * splits)), dim3(kBlock), 0, as_stream(stream),      \
-                     (const T*)X, ldx, cols, (int)splits, c, inv_t, k, t64, t32, ignore_index, top_idx,                  \
-                     (const float4*)stats, glogp, gentropy, gtop, (T*)GX)
-#define LP_BWD(T)                                                                         \
-  const int64_t splits = (cols + kBlock * NV * Vec<T>::N - 1) / (kBlock * NV * Vec<T>::N); \
-  if (cols % Vec<T>::N == 0) LP_BWD_F(T, true);                                           \
-  else LP_BWD_F(T, false)
+#define LP_BWD_F(T, L, F)                                                                                                \
+  hipLaunchKernelGGL((lp_bwd_kernel<T, L, NV, F>), dim3((unsigned)((rows * splits + kBlock / L - 1) / (kBlock / L))),     \
+                     dim3(kBlock), 0, as_stream(stream), (const T*)X, ldx, rows, cols, (int)splits, c, inv_t, k, t64,     \
+                     t32, ignore_index, top_idx, (const float4*)stats, glogp, gentropy, gtop, (T*)GX)
+#define LP_BWD_L(T, L)                                                          \
+  do {                                                                          \
+    const int64_t len = L * NV * Vec<T>::N, splits = (cols + len - 1) / len;    \
+    if (cols % Vec<T>::N == 0) LP_BWD_F(T, L, true);                            \
+    else LP_BWD_F(T, L, false);                                                 \
+  } while (0)
+#define LP_BWD(T)                                        \
+  do {                                                   \
+    if (short_rows(rows, cols)) LP_BWD_L(T, 64);         \
+    else LP_BWD_L(T, kBlock);                            \
+  } while (0)
   MMSSL_BY_DTYPE(dtype, LP_BWD);
   MMSSL_LAUNCH_CHECK();
   return 0;

@@ -411,6 +411,23 @@ def test_logprobs_many_rows_whole_slices_and_one_launch(t):
     check_logprobs(scores(260, 17000, t, 4), k=3)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols", [(2048, 1), (2050, 100), (2049, 511), (2051, 1000), (3001, 1025), (2048, 2048),
+                                       (2047, 700), (2048, 2049)])
+def test_logprobs_many_short_rows(rows, cols, t):
+    """Rows that a wave takes alone, forward and backward, and their neighbours that a block takes; a masked row, an empty one,
+    one with a NaN among them."""
+    x = scores(rows, cols, t, rows + cols, masked=0.2)
+    x[5] = float("-inf")
+    x[7] = torch.finfo(t).min
+    check_logprobs(x, k=0, temperature=1.7)
+    check_logprobs(x[:, :cols], k=min(3, cols))
+    from mmssl_amd import ops
+    x[rows - 1, cols // 2] = float("nan")
+    o = ops.logprobs_rows(x.to(DEV), torch.zeros(rows, dtype=torch.int64, device=DEV))
+    assert bool(o[0][-1].isnan()) and bool(o[1][-1].isnan()) and not bool(o[1][:-1].isnan().any())
+
+
 @pytest.mark.parametrize("cols", [100, 900, 3000, 70000])
 def test_logprobs_rows_of_equal_and_masked_values(cols):
     """Ties go to the lowest column, whatever their number; rows that the mask leaves little or nothing of; masks of the
