@@ -756,7 +756,7 @@ int mmssl_embed_rows_bwd(const void* g, int64_t ldg, int dtype, const void* idx,
 /* Layer norm over the rows of X [rows, d] (csrc/layernorm.hip): Y = (x - mean) / sqrt(var + eps) * weight + bias, var the mean
  * square around the mean. X row r starts at X + r * ldx (ldx = 0: one row for all), Y is contiguous. weight and bias (either
  * may be NULL: 1 and 0) hold d numbers of type param_dtype. stats (may be NULL): [rows][2] fp32, mean and 1 / sqrt(var + eps)
- * of each row, for the backward pass. d <= 2^24. */
+ * of each row, for the backward pass. d <= 2^24; rows < 2^22 where d > 16384. */
 int mmssl_layernorm_rows(const void* X, int64_t ldx, int dtype, int64_t rows, int d, const void* weight, const void* bias,
                          int param_dtype, float eps, void* Y, float* stats, void* stream);
 /* Its gradients: GX [rows, d] contiguous, gweight and gbias [d] of type param_dtype, each of which may be NULL (not wanted).
@@ -773,7 +773,8 @@ int mmssl_layernorm_rows_bwd(const void* X, int64_t ldx, const void* G, int64_t 
  * target: int32 (target_bytes 4) or int64 (8); a target equal to ignore_index gives logp 0, any other outside [0, cols) NaN.
  * An entry of -inf has probability 0 (and -inf as its logp); a row of nothing else has entropy 0 and logp -inf. A NaN or
  * +inf in a row makes its logp and entropy NaN; NaN ranks above +inf. stats (may be NULL): [rows][4] fp32, 16-byte aligned,
- * for the backward pass. k <= cols <= 2^31 - 16. The workspace (16-byte aligned) need not be cleared. */
+ * for the backward pass. k <= cols <= 2^31 - 16, rows * ceil(cols / 2048) < 2^24. The workspace (16-byte aligned) need not be
+ * cleared. */
 size_t mmssl_logprobs_rows_workspace_bytes(int dtype, int64_t rows, int64_t cols, int k);
 int mmssl_logprobs_rows(const void* X, int64_t ldx, int dtype, int64_t rows, int64_t cols, const void* target,
                         int target_bytes, int64_t ignore_index, int k, float temperature, float* logp, float* entropy,

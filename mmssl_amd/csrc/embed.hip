@@ -508,7 +508,7 @@ int grad_launch(const int2* KP, int64_t n, int rows, int d, const T* g, int64_t 
   const int64_t rblocks = groups * ctiles;
   const int zrows = (int)std::max<int64_t>(32, std::min<int64_t>(kZeroRowsMax, (64 << 10) / ((int64_t)d * sizeof(T))));
   const int64_t zblocks = ((int64_t)rows + zrows - 1) / zrows;
-  if (rblocks + zblocks > 0x7fffffff) return MMSSL_E_UNSUPP;
+  if (!launchable(rblocks + zblocks, kBlock)) return MMSSL_E_UNSUPP;
   if (rblocks + zblocks == 0) return 0;
   hipLaunchKernelGGL((embed_grad_kernel<T, LPR, FULL>), dim3((unsigned)(rblocks + zblocks)), dim3(kBlock), 0, s, KP, n, rows, d,
                      g, ldg, scale, gW, part, p.chunk, p.chunks, ctiles, rblocks, zrows);
@@ -559,7 +559,7 @@ extern "C" int mmssl_embed_rows(const void* table, int64_t ldt, int dtype, int64
     else if (full) { EMBED_FWD_F(T, int32_t, true); }        \
     else { EMBED_FWD_F(T, int32_t, false); }                 \
   } while (0)
-  if (blocks > 0x7fffffff) return MMSSL_E_UNSUPP;
+  if (!launchable(blocks, kBlock)) return MMSSL_E_UNSUPP;
   MMSSL_BY_DTYPE(dtype, EMBED_FWD);
   MMSSL_LAUNCH_CHECK();
   return 0;

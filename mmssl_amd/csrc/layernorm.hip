@@ -434,7 +434,7 @@ int64_t parts_for(int64_t rows, int d, int es) {
 int check_common(int dtype, int64_t rows, int d, int pdt, float eps) {
   if (!known_dtype(dtype) || !known_dtype(pdt) || rows < 0 || d < 1 || !(eps >= 0.f)) return MMSSL_E_BADARG;
   // one block a row where rows are wide; a row's columns are counted in 32 bits
-  if (d > (1 << 24) || (d > kMaxInRegs && rows > 0x7fffffff)) return MMSSL_E_UNSUPP;
+  if (d > (1 << 24) || (d > kMaxInRegs && !launchable(rows, kWideThreads))) return MMSSL_E_UNSUPP;
   return 0;
 }
 

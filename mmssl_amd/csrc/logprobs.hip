@@ -644,8 +644,8 @@ int check_common(int dtype, int64_t rows, int64_t cols, int target_bytes, int k,
   if (!known_dtype(dtype) || rows < 0 || cols < 1 || (target_bytes != 4 && target_bytes != 8) || k < 0) return MMSSL_E_BADARG;
   if (!(temperature > 0.f) || temperature > 3.0e38f || !(1.0f / temperature <= 3.0e38f)) return MMSSL_E_BADARG;
   if (k > kTopMax || k > cols || cols > 0x7ffffff0) return MMSSL_E_UNSUPP;
-  // blocks of a launch; a row's pairs (at most cols / 2048 + 1 slices of k) are counted in 32 bits
-  if (rows * ((cols + 2047) / 2048) > 0x3fffffff) return MMSSL_E_UNSUPP;
+  // a row's slices are no shorter than 2048 columns (but for the last), so its pairs are counted in 32 bits
+  if (rows > 0x7fffffff || !launchable(rows * ((cols + 2047) / 2048), kBlock)) return MMSSL_E_UNSUPP;
   return 0;
 }
 

@@ -50,6 +50,7 @@ PyObject* g_error = nullptr;
 struct Lib {
 #define MMSSL_MEMBER(f) decltype(&f) p_##f = nullptr;
   MMSSL_BOUND(MMSSL_MEMBER)
+  hipError_t (*is_capturing)(hipStream_t, hipStreamCaptureStatus*) = nullptr;      // the runtime's that the library runs on
 } lib;
 #define CALL(f) lib.p_##f
 
@@ -59,6 +60,8 @@ void bind(uintptr_t handle, py::object error) {
   l.p_##f = reinterpret_cast<decltype(l.p_##f)>(dlsym(reinterpret_cast<void*>(handle), #f));    \
   if (!l.p_##f) throw std::runtime_error("libmmssl_hip.so does not export " #f " (stale build?)");
   MMSSL_BOUND(MMSSL_RESOLVE)
+  l.is_capturing = reinterpret_cast<decltype(l.is_capturing)>(dlsym(reinterpret_cast<void*>(handle), "hipStreamIsCapturing"));
+  if (!l.is_capturing) throw std::runtime_error("no hipStreamIsCapturing among the libraries of libmmssl_hip.so");
   lib = l;
   Py_XDECREF(g_error);
   g_error = error.inc_ref().ptr();
@@ -84,6 +87,10 @@ void same_device(const Tensor& t, const Tensor& other, const char* name) {
     refuse(std::string(name) + " is on " + other.device().str() + ", expected " + t.device().str());
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+bool capturing(const Tensor& t) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  return lib.is_capturing(static_cast<hipStream_t>(stream_of(t)), &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+}
 Tensor bytes_on(const Tensor& t, size_t n) { return at::empty({(int64_t)n}, t.options().dtype(at::kByte)); }
 std::string shape_of(at::IntArrayRef s) {
   std::string r = "[";
@@ -115,6 +122,19 @@ void first_order(const char* what) {
 }
 bool records(const Tensor& a) { return a.defined() && a.requires_grad(); }
 
+// Recorded inside a capture, with an input whose part of the graph (its producer, or the accumulator that an eager graph of the
+// same leaf keeps alive) belongs to the default stream: the engine would make the capture wait for that stream, which cannot be
+// captured. The engine's threads do not come back from that, so it is refused here.
+void recordable(const Tensor& input, const char* what) {
+  if (!records(input)) return;
+  const auto node = input.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(input) : input.grad_fn();
+  if (!node) return;
+  const auto s = node->stream();
+  if (s && s->id() == c10::hip::getDefaultHIPStream(input.device().index()).id() && capturing(input))
+    refuse(std::string(what) + ": a captured backward pass cannot reach into an eager graph of the default stream: run the " +
+           "warm-up on the capture's own stream and release its graph, or capture under torch.no_grad()");
+}
+
 // int32 / int64 numbers on t's device, contiguous; host tensors are uploaded
 Tensor tokens(const Tensor& t, Tensor idx, const char* name) {
   const auto s = idx.scalar_type();
@@ -122,6 +142,7 @@ Tensor tokens(const Tensor& t, Tensor idx, const char* name) {
     refuse(std::string(name) + " must hold int64 or int32 numbers, got " + toString(s));
   if (idx.device() != t.device()) {
     if (idx.is_cuda()) same_device(t, idx, name);
+    if (capturing(t)) refuse(std::string(name) + ": host tensors cannot be uploaded while a graph is captured");
     idx = idx.to(t.device());
   }
   return idx.contiguous();
@@ -180,7 +201,10 @@ Tensor embed_rows(const Tensor& table, const Tensor& idx_, double scale, std::op
   fits_int(table.size(1), "embed_rows");
   const Tensor idx = tokens(table, idx_, "idx");
   const Pad pad{padding_idx.has_value(), padding_idx.value_or(0)};
-  if (at::GradMode::is_enabled() && records(table)) return EmbedRows::apply(table, idx, scale, pad.has, pad.idx);
+  if (at::GradMode::is_enabled() && records(table)) {
+    recordable(table, "embed_rows");
+    return EmbedRows::apply(table, idx, scale, pad.has, pad.idx);
+  }
   return embed_forward(table, idx, scale, pad);
 }
 
@@ -256,6 +280,7 @@ Tensor layernorm_rows(const Tensor& X, const std::optional<Tensor>& weight, cons
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
     refuse("layernorm_rows: weight and bias must be of one type");
   if (at::GradMode::is_enabled() && (records(X) || records(w) || records(b))) {
+    for (const Tensor* t : {&X, &w, &b}) recordable(*t, "layernorm_rows");
     auto there = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     return LayerNormRows::apply(X, there(w), there(b), eps);
   }
@@ -343,9 +368,10 @@ py::tuple logprobs_rows(const Tensor& X, const Tensor& target_, int64_t k, doubl
   const auto lead = X.sizes().slice(0, X.dim() - 1);
   if (target.sizes() != lead)
     refuse("logprobs_rows: target must be " + shape_of(lead) + ", got " + shape_of(target.sizes()));
-  const variable_list out = at::GradMode::is_enabled() && records(X)
-                                ? LogprobsRows::apply(X, target, k, temperature, ignore)
-                                : logprobs_forward(X, target, k, temperature, ignore, nullptr);
+  const bool record = at::GradMode::is_enabled() && records(X);
+  if (record) recordable(X, "logprobs_rows");
+  const variable_list out = record ? LogprobsRows::apply(X, target, k, temperature, ignore)
+                                   : logprobs_forward(X, target, k, temperature, ignore, nullptr);
   if (!k) return py::make_tuple(out[0], out[1], py::none(), py::none());
   return py::make_tuple(out[0], out[1], out[2], out[3]);
 }

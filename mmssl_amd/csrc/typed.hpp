@@ -76,6 +76,9 @@ inline bool known_dtype(int t) { return t == MMSSL_F32 || t == MMSSL_BF16 || t =
 inline int dtype_bytes(int t) { return t == MMSSL_F32 ? 4 : 2; }
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// a launch counts its threads in 32 bits
+inline bool launchable(int64_t blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
+
 // CALL(T) once, with the element type of code DT
 #define MMSSL_BY_DTYPE(DT, CALL)        \
   do {                                  \

@@ -1449,6 +1449,7 @@ def logprobs_rows(X, target, k=0, temperature=1.0, ignore_index=-100):
     None for k = 0). fp32 results with fp32 sums; X is read once, n * rows probabilities are never stored.
     Masked columns hold -inf: probability 0. A row of nothing else has logp -inf, entropy 0, gradient 0. `ignore_index` as a
     target: logp 0; any other target outside the row: logp NaN; neither has a gradient. A NaN or +inf in a row makes its logp
-    and entropy NaN. Differentiable in X through logp, entropy and top_logp."""
+    and entropy NaN. Differentiable in X through logp, entropy and top_logp. Up to 2^24 - 1 rows of up to 2048 columns (of longer
+    ones as many fewer)."""
     _given(X, "X")
     return _lib.binding().logprobs_rows(X, _numbers(target), k, temperature, ignore_index)

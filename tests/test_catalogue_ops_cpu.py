@@ -107,6 +107,23 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.mmssl_grad_norm_workspace_bytes(-1) == 0
 
 
+def test_launches_past_32_bits_of_threads_are_refused():
+    from mmssl_amd import _lib
+    L = _lib.lib()
+    p = 1 << 20
+    lp = [p, 100, 0, 1 << 24, 100, p, 8, -100, 0, 1.0, p, p, p, p, p, p, 1 << 40, None]
+    assert L.mmssl_logprobs_rows(*lp) == UNSUPP
+    assert L.mmssl_logprobs_rows_bwd(p, 100, 0, 1 << 24, 100, p, 8, -100, 0, 1.0, p, p, p, p, None, p, None) == UNSUPP
+    assert L.mmssl_logprobs_rows_workspace_bytes(0, 1 << 24, 100, 0) == 0
+    assert L.mmssl_logprobs_rows_workspace_bytes(0, (1 << 24) - 1, 100, 0) > 0
+    assert L.mmssl_logprobs_rows_workspace_bytes(0, 1 << 23, 2049, 0) == 0
+    assert L.mmssl_logprobs_rows_workspace_bytes(0, 1 << 62, 1, 0) == 0
+    assert L.mmssl_layernorm_rows(p, 20000, 1, 1 << 22, 20000, p, p, 0, 1e-5, p, p, None) == UNSUPP
+    assert L.mmssl_layernorm_rows_bwd(p, 20000, p, 20000, 1, 1 << 22, 20000, p, 0, p, p, None, None, None, 0, None) == UNSUPP
+    # 16 rows a block above 64 vectors a row
+    assert L.mmssl_embed_rows(p, 1000, 0, 10, 1000, p, 8, 1 << 29, 1.0, 0, 0, p, 1000, None) == UNSUPP
+
+
 def test_missing_binding_fails_loudly():
     import os
     import subprocess

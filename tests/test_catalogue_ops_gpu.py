@@ -770,6 +770,48 @@ def test_catalogue_operators_in_a_captured_graph():
                 assert torch.equal(a, b), (turn, k, i)
 
 
+def test_capture_refuses_what_the_capture_could_not_hold():
+    """A leaf of a live eager graph of the default stream, a producer of one, numbers on the host: an error before anything is
+    recorded; the same calls are captured once the eager graph is gone, or without gradients."""
+    from mmssl_amd import ops
+    from mmssl_amd._lib import MmsslError
+    w = torch.randn(50, 64, device=DEV, requires_grad=True)
+    v = torch.randn(64, device=DEV, requires_grad=True)
+    idx = torch.arange(20, device=DEV)
+    rows = w.detach()[:20]
+    eager = ops.layernorm_rows(ops.embed_rows(w, idx), v)                # kept: holds the accumulators of w and v
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+
+    def captured(fn):
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
+            out = fn()
+        return g, out
+
+    for name, fn in (("leaf", lambda: ops.embed_rows(w, idx)), ("parameter", lambda: ops.layernorm_rows(rows, v)),
+                     ("producer", lambda: ops.layernorm_rows(eager)), ("scores", lambda: ops.logprobs_rows(eager, idx)),
+                     ("tokens", lambda: ops.embed_rows(w.detach(), [1, 2, 3])),
+                     ("target", lambda: ops.logprobs_rows(rows, torch.zeros(20, dtype=torch.int64)))):
+        print(name, flush=True)
+        with pytest.raises(MmsslError):
+            captured(fn)
+    with torch.no_grad():
+        g, out = captured(lambda: ops.layernorm_rows(ops.embed_rows(w, idx), v))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, eager.detach())
+    want = torch.autograd.grad(eager, (w, v), torch.ones_like(eager))
+    one = torch.ones_like(eager).detach()
+    del eager
+    g, got = captured(lambda: torch.autograd.grad(ops.layernorm_rows(ops.embed_rows(w, idx), v), (w, v), one))
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_catalogue_operators_on_two_streams_at_once():
     from mmssl_amd import ops, optim
     g0 = gen(71)
