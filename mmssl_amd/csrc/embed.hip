@@ -72,8 +72,9 @@ __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(const T* __restrict__
   }
 }
 
-// Rows of up to 64 vectors: a block's threads share the vectors of its tokens evenly, whatever their number a row (lane groups of
-// a power of two leave half the lanes idle at width 65: 20 M fp32 values 38 us, so 30; at width 64 the same 25).
+// Rows of up to 64 vectors that do not fill a lane group of a power of two: a block's threads share the vectors of its tokens
+// evenly (20 M fp32 values at width 65: lane groups 38 us, so 30; where the groups are full they are faster, 1 M rows of 128
+// bf16: 82 against 93 us).
 // magic = ceil(2^20 / vecs): (l * magic) >> 20 = l / vecs for every l < kFlat = 2^10 (the error l * 64 stays below 2^20, the
 // product at or below 2^30).
 constexpr int kFlatU = 4, kFlat = kBlock * kFlatU;
@@ -539,18 +540,23 @@ extern "C" int mmssl_embed_rows(const void* table, int64_t ldt, int dtype, int64
   const size_t es = dtype_bytes(dtype);
   if (!aligned_to(table, es) || !aligned_to(out, es) || !aligned_to(idx, idx_bytes)) return MMSSL_E_BADARG;
   const IdxRule q{(int)rows, has_padding ? 1 : 0, padding_idx};
-  const int vecs = (int)((d + 16 / es - 1) / (16 / es));
+  const int vecs = (int)((d + 16 / es - 1) / (16 / es)), lpr = lanes_for(vecs);
+  const bool flat = vecs < lpr;
   constexpr int U = 4;
-  const int tokens = vecs <= 64 ? kFlat / vecs : kBlock / 64 * U;           // of a block
+  const int tokens = flat ? kFlat / vecs : kBlock / lpr * U;                // of a block
   const int64_t blocks = (n + tokens - 1) / tokens;
   const uint32_t magic = ((1u << 20) + vecs - 1) / vecs;
+#define EMBED_FWD_L(T, I, L, F)                                                                                          \
+  hipLaunchKernelGGL((embed_fwd_kernel<T, I, L, U, F>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),       \
+                     (const T*)table, ldt, d, (const I*)idx, n, q, scale, (T*)out, ldo)
 #define EMBED_FWD_F(T, I, F)                                                                                             \
-  if (vecs <= 64)                                                                                                        \
+  if (flat)                                                                                                              \
     hipLaunchKernelGGL((embed_fwd_flat_kernel<T, I, F>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),      \
                        (const T*)table, ldt, d, vecs, magic, tokens, (const I*)idx, n, q, scale, (T*)out, ldo);          \
-  else                                                                                                                   \
-    hipLaunchKernelGGL((embed_fwd_kernel<T, I, 64, U, F>), dim3((unsigned)blocks), dim3(kBlock), 0, as_stream(stream),    \
-                       (const T*)table, ldt, d, (const I*)idx, n, q, scale, (T*)out, ldo)
+  else if (lpr == 8) EMBED_FWD_L(T, I, 8, F);                                                                            \
+  else if (lpr == 16) EMBED_FWD_L(T, I, 16, F);                                                                          \
+  else if (lpr == 32) EMBED_FWD_L(T, I, 32, F);                                                                          \
+  else EMBED_FWD_L(T, I, 64, F)
 #define EMBED_FWD(T)                                         \
   do {                                                       \
     const bool full = d % Vec<T>::N == 0;                    \
