@@ -770,6 +770,31 @@ def test_catalogue_operators_in_a_captured_graph():
                 assert torch.equal(a, b), (turn, k, i)
 
 
+@pytest.mark.parametrize("d", [8, 20, 64, 300])
+@pytest.mark.parametrize("kind", ["one", "half", "steep", "two"])
+def test_embed_gradient_of_popular_tokens(kind, d):
+    """Tokens that hold a large part of 300 001 places: their chunks are counted by a search, their partial rows joined by a whole
+    block, and the rows without a place among them found by a search. fp32 sums: chunks of up to 64 places, then the chunks' sums
+    over 4 to 32 groups, so no entry passes through more than 64 + 4688 / 4 + 32 additions; the same call gives the same bits."""
+    from mmssl_amd import ops
+    n, rows = 300001, 3001
+    q = gen(d)
+    u = torch.rand(n, generator=q)
+    idx = {"one": torch.full((n,), 1500), "half": torch.where(u < 0.5, 7, (u * 3000).long()),
+           "steep": (rows * u ** 6).long().clamp_(0, rows - 1), "two": torch.where(u < 0.4, 0, 3000)}[kind].long()
+    g = torch.randn(n, d, generator=q)
+    w = torch.zeros(rows, d, device=DEV, requires_grad=True)
+    out = ops.embed_rows(w, idx.to(DEV))
+    (a,) = torch.autograd.grad(out, w, g.to(DEV), retain_graph=True)
+    (b,) = torch.autograd.grad(out, w, g.to(DEV))
+    assert torch.equal(a, b)
+    want = torch.zeros(rows, d, dtype=torch.float64).index_add_(0, idx, g.double())
+    size = torch.zeros(rows, d, dtype=torch.float64).index_add_(0, idx, g.double().abs())
+    err = (a.cpu().double() - want).abs()
+    assert bool((err <= 1300 * 2.0 ** -24 * size).all()), float((err / size.clamp_min(1e-30)).max())
+    assert bool((a.cpu()[size[:, 0] == 0] == 0).all())
+
+
 def test_capture_refuses_what_the_capture_could_not_hold():
     """A leaf of a live eager graph of the default stream, a producer of one, numbers on the host: an error before anything is
     recorded; the same calls are captured once the eager graph is gone, or without gradients."""
