@@ -88,6 +88,12 @@ def test_embed_gradient_of_long_lists_is_sorted_by_radix(rows, n):
     assert torch.equal(got, check_embed(rows, 8, idx, torch.bfloat16, seed=4)), "the same call, the same bits"
 
 
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 9216, 9217])
+def test_embed_gradient_where_ranking_ends(n):
+    for rows in (1, 255, 256, 65537):
+        check_embed(rows, 12, torch.randint(rows, (n,), generator=gen(n + rows)), torch.float32, seed=n)
+
+
 def test_embed_popular_tokens_cross_many_chunks():
     """Tokens whose places fill one chunk, several, more than one lane group joins alone, and the whole list."""
     for counts in ([1, 7, 8, 9, 64, 65, 200, 1000, 0, 3], [5000], [1, 0, 0, 4000, 1], [8, 8, 8, 8], [16, 0, 128, 129, 127]):
@@ -234,6 +240,14 @@ def test_layernorm_gradients_of_many_rows(rows, d, t):
     a = check_norm((rows, d), t, seed=rows)
     b = check_norm((rows, d), t, seed=rows)
     assert all(torch.equal(x, y) for x, y in zip(a, b)), "the same call, the same bits"
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,d", [(2100, 5), (2100, 9), (1500, 77), (1300, 131), (1100, 257), (700, 513), (600, 1001),
+                                    (560, 2051), (530, 4097), (520, 8193)])
+def test_layernorm_rows_that_end_inside_a_vector(rows, d, t):
+    """One to seven columns behind the last whole vector, at every lane group and number of vectors a lane."""
+    check_norm((rows, d), t, seed=d)
 
 
 def test_layernorm_parameters_types_and_absence():
