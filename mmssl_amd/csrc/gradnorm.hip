@@ -87,38 +87,43 @@ struct Walk {
   }
 };
 
-// Lists in the workspace: a block's chunks follow each other; one search for the first by all threads at once (entries
-// counted whose first chunk is not behind it), then the entry stays in registers until its chunks end.
+// Lists in the workspace: a block's chunks follow each other. Where they are is worked out for kAhead of them at a time: each
+// thread looks at its share of the entries and writes down the chunks that fall into its entries, so that the entries are one
+// round of loads and not a chain of them in front of every tensor (600 tensors, 60 M bf16: both launches 86 us, so 80).
 struct Table {
   const Entry* e;
   int32_t count, chunks;
 };
+constexpr int kAhead = 64;
 template <>
 struct Walk<Table> {
   const Table l;
-  int at = -1, until = -1;                // the entry at hand, the chunk behind its last
-  Entry cur;
-  __device__ __forceinline__ Walk(const Table& table) : l(table) {}
+  Place* at;                              // LDS, kAhead of them
+  int from = 0, until = 0;                // the chunks that are there
+  __device__ __forceinline__ Walk(const Table& table) : l(table) {
+    __shared__ Place place[kAhead];
+    at = place;
+  }
   __device__ __forceinline__ int begin(int chunks) const { return (int)((int64_t)chunks * blockIdx.x / gridDim.x); }
   __device__ __forceinline__ int end(int chunks) const { return (int)((int64_t)chunks * (blockIdx.x + 1) / gridDim.x); }
   __device__ __forceinline__ int step() const { return 1; }
   __device__ __forceinline__ int from_back(int i, int) const { return i; }
-  __device__ __forceinline__ Place find(int chunk) {
+  __device__ __forceinline__ Place find(int chunk) {             // the same chunk for every thread of the block
     if (chunk >= until) {
-      if (at < 0) {
-        int n = 0;
-        for (int i = 0; i < l.count; i += kBlock) {              // every thread of the block takes part
-          const int k = i + (int)threadIdx.x;
-          n += __syncthreads_count(k < l.count && l.e[k].first <= chunk);
-        }
-        at = n - 1;
-      } else {
-        while (at + 1 < l.count && l.e[at + 1].first <= chunk) ++at;
+      from = chunk;
+      until = min(chunk + kAhead, end(l.chunks));
+      __syncthreads();
+#pragma unroll 4
+      for (int i = threadIdx.x; i < l.count; i += kBlock) {
+        const Entry e = l.e[i];
+        const int last = e.first + (int)((e.n + kChunk - 1) / kChunk);
+        for (int c = max(e.first, from); c < min(last, until); ++c) at[c - from] = place_of(e.g, e.o, e.n, e.dt, c - e.first);
       }
-      cur = l.e[at];
-      until = cur.first + (int)((cur.n + kChunk - 1) / kChunk);
+      __syncthreads();
     }
-    return place_of(cur.g, cur.o, cur.n, cur.dt, chunk - cur.first);
+    Place p = at[chunk - from];
+    p.dt = __builtin_amdgcn_readfirstlane(p.dt);
+    return p;
   }
 };
 template <class L>

@@ -965,6 +965,25 @@ def test_modes_without_gradients_and_changed_inputs():
     assert float(gx.abs().max()) < 1e-4                       # the rows' gradients of a plain sum cancel
 
 
+def test_long_gradient_lists_of_more_chunks_than_a_block_looks_ahead():
+    """97 tensors of 560 M elements: a block has more chunks than it works out at once. The squares are whole numbers, so the norm
+    is exact up to its last rounding, and the factor 2^-8 is as well."""
+    from mmssl_amd import optim
+    sizes = [5_770_000 + 37 * i for i in range(96)] + [1_000_003]
+    grads = [torch.full((n,), 1.0 + i % 3, device=DEV, dtype=torch.bfloat16) for i, n in enumerate(sizes)]
+    for i, g in enumerate(grads):
+        g[-1] = 200.0 + i                                                 # (rounded by the type)
+    total = sum(int(g[-1]) ** 2 + (n - 1) * (1 + i % 3) ** 2 for i, (n, g) in enumerate(zip(sizes, grads)))
+    norm = total ** 0.5
+    out = [torch.empty_like(g) for g in grads]
+    got = optim.clip_grads(grads, norm / 256, out=out)
+    assert abs(float(got) - norm) <= 2 ** -23 * norm
+    for g, o in zip(grads, out):
+        # the factor is 2^-8 up to a few half steps of 32 bits, far below one of bf16
+        assert bool((o.float() - g.float() / 256).abs().max() <= float(g.max()) / 256 * 2 ** -8)
+        assert torch.equal(o[0].float() * 256, g[0].float()) and torch.equal(o[-1].float() * 256, g[-1].float())
+
+
 def test_long_gradient_lists_in_captured_graphs():
     """Lists past the kernel arguments' go through a table in the workspace: two graphs with their own, replayed in turn with
     eager calls between them."""
