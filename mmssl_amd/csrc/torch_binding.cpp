@@ -75,8 +75,15 @@ void check(int rc, const char* what) {
 int dtype_code(at::ScalarType t) {
   return t == at::kFloat ? MMSSL_F32 : t == at::kBFloat16 ? MMSSL_BF16 : t == at::kHalf ? MMSSL_F16 : -1;
 }
+// A tangent of forward-mode differentiation on an operand: the operators have no such derivative, and their outputs would come
+// out as if it were zero. (Undefined where the mode is off.)
+void no_tangent(const Tensor& t, const char* name) {
+  if (t.defined() && t._fw_grad(/*level=*/0).defined())
+    refuse(std::string(name) + " carries a forward-mode tangent: only reverse-mode derivatives are there");
+}
 int typed(const Tensor& t, const char* name) {
   if (!t.is_cuda()) refuse(std::string(name) + " must be a CUDA (HIP) tensor: this package has no CPU path");
+  no_tangent(t, name);
   const int c = dtype_code(t.scalar_type());
   if (c < 0 || t.layout() != at::kStrided)
     refuse(std::string(name) + " must be a dense float32, bfloat16 or float16 tensor, got " + toString(t.scalar_type()));
@@ -116,9 +123,10 @@ void fits_int(int64_t d, const char* what) {
   if (d > (1 << 24)) refuse(std::string(what) + ": rows of at most 2^24 columns, got " + std::to_string(d));
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-void first_order(const char* what) {
+void first_order(const char* what, const variable_list& grads) {
   if (at::GradMode::is_enabled())            // the engine enables it only for create_graph=True
     refuse(std::string(what) + ": the gradient is not differentiable again");
+  for (const Tensor& g : grads) no_tangent(g, what);
 }
 bool records(const Tensor& a) { return a.defined() && a.requires_grad(); }
 
@@ -176,7 +184,7 @@ struct EmbedRows : torch::autograd::Function<EmbedRows> {
     return embed_forward(table, idx, scale, {has_pad, pad});
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    first_order("embed_rows");
+    first_order("embed_rows", grads);
     const Tensor idx = ctx->get_saved_variables()[0];
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
     const int64_t rows = cfg[0], d = cfg[1];
@@ -235,7 +243,7 @@ struct LayerNormRows : torch::autograd::Function<LayerNormRows> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    first_order("layernorm_rows");
+    first_order("layernorm_rows", grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &X = saved[0], &w = saved[1], &stats = saved[2];
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
@@ -331,7 +339,7 @@ struct LogprobsRows : torch::autograd::Function<LogprobsRows> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    first_order("logprobs_rows");
+    first_order("logprobs_rows", grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &X = saved[0], &target = saved[1], &stats = saved[2], &top_idx = saved[3];
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
@@ -389,6 +397,7 @@ GradList list_of(const std::vector<Tensor>& ts, const char* what, c10::Device de
   l.dtype.reserve(ts.size());
   for (const Tensor& t : ts) {
     if (!t.defined() || t.layout() != at::kStrided) refuse(std::string(what) + ": dense tensors expected");
+    no_tangent(t, what);
     if (!t.is_cuda() || t.device() != dev)
       refuse(std::string(what) + ": gradients must be on one CUDA (HIP) device: this package has no CPU path");
     const int c = dtype_code(t.scalar_type());

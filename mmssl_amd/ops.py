@@ -1409,7 +1409,8 @@ def ngcf_combine(G, B, keep=None, scale=1.0):
 
 # ---------------------------------------------------------------------------------------
 # Operators of a full-catalogue softmax model (csrc/embed.hip, layernorm.hip, logprobs.hip): fp32, bf16 and fp16. Checks,
-# output tensors and autograd nodes are in csrc/torch_binding.cpp.
+# output tensors and autograd nodes are in csrc/torch_binding.cpp. Their derivatives are the reverse-mode ones, once: a tensor
+# with a forward-mode tangent and a backward pass under create_graph=True are refused.
 # ---------------------------------------------------------------------------------------
 def _given(t, name):
     if not isinstance(t, torch.Tensor):

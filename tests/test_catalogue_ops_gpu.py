@@ -1010,3 +1010,44 @@ def test_long_gradient_lists_in_captured_graphs():
             torch.cuda.synchronize()
             assert torch.equal(norm, eager)
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_forward_mode_tangents_are_refused():
+    """An operand or an incoming gradient with a tangent: there is no such derivative, and none may come out as zero."""
+    from torch.autograd import forward_ad as fw
+    from mmssl_amd import ops, optim
+    from mmssl_amd._lib import MmsslError
+    x = torch.randn(6, 40, device=DEV)
+    idx = torch.arange(6, device=DEV)
+    w = torch.ones(40, device=DEV)
+    with fw.dual_level():
+        def dual(v):
+            return fw.make_dual(v, torch.ones_like(v))
+        for base in (x, x.clone().requires_grad_(True)):
+            for fn in (lambda: ops.embed_rows(dual(base), idx), lambda: ops.layernorm_rows(dual(base)),
+                       lambda: ops.layernorm_rows(base, dual(w)), lambda: ops.layernorm_rows(base, None, dual(w)),
+                       lambda: ops.layernorm_rows(base, w, dual(w)), lambda: ops.logprobs_rows(dual(base), idx),
+                       lambda: ops.logprobs_rows(dual(base), idx, k=3)):
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(MmsslError, match="forward-mode"):
+                        fn()
+        y = x.clone()
+        for fn in (lambda: optim.grad_norm([y, dual(y)]), lambda: optim.clip_grads([dual(y)], 0.1),
+                   lambda: optim.clip_grads([y], 0.1, out=[dual(torch.zeros_like(y))])):
+            with pytest.raises(MmsslError, match="forward-mode"):
+                fn()
+        assert torch.equal(y, x)
+        leaf = x.clone().requires_grad_(True)
+        for fn in (lambda: ops.embed_rows(leaf, idx), lambda: ops.layernorm_rows(leaf),
+                   lambda: ops.logprobs_rows(leaf, idx)[0], lambda: ops.logprobs_rows(leaf, idx)[1],
+                   lambda: ops.logprobs_rows(leaf, idx, k=3)[2]):
+            out = fn()
+            one = torch.ones_like(out)
+            want = torch.autograd.grad(out, leaf, one, retain_graph=True)[0]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, dual(one), retain_graph=True)
+            assert torch.equal(torch.autograd.grad(out, leaf, one)[0], want)
+        held = dual(x)
+        want = ops.layernorm_rows(x)
+        assert torch.equal(ops.layernorm_rows(fw.unpack_dual(held).primal), want)
+    assert torch.equal(ops.layernorm_rows(held), want)                    # the level is gone, and the tangent with it
