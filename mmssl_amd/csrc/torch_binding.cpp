@@ -130,17 +130,28 @@ void first_order(const char* what, const variable_list& grads) {
 }
 bool records(const Tensor& a) { return a.defined() && a.requires_grad(); }
 
-// Recorded inside a capture, with an input whose part of the graph (its producer, or the accumulator that an eager graph of the
-// same leaf keeps alive) belongs to the default stream: the engine would make the capture wait for that stream, which cannot be
-// captured. The engine's threads do not come back from that, so it is refused here.
+// Recorded inside a capture, with an input from which the graph reaches a node of the default stream: an eager producer, or the
+// accumulator that an eager graph of the same leaf keeps alive, however many nodes of the capture lie between. The engine would
+// make the capture wait for that stream, which cannot be captured. The engine's threads do not come back from that, so it is
+// refused here. (What the caller joins to the output afterwards is out of sight.)
 void recordable(const Tensor& input, const char* what) {
   if (!records(input)) return;
-  const auto node = input.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(input) : input.grad_fn();
-  if (!node) return;
-  const auto s = node->stream();
-  if (s && s->id() == c10::hip::getDefaultHIPStream(input.device().index()).id() && capturing(input))
-    refuse(std::string(what) + ": a captured backward pass cannot reach into an eager graph of the default stream: run the " +
-           "warm-up on the capture's own stream and release its graph, or capture under torch.no_grad()");
+  const auto none = c10::hip::getDefaultHIPStream(input.device().index()).id();
+  if (c10::hip::getCurrentHIPStream(input.device().index()).id() == none || !capturing(input)) return;
+  const auto root = input.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(input) : input.grad_fn();
+  if (!root) return;
+  std::vector<torch::autograd::Node*> todo{root.get()};
+  std::unordered_set<torch::autograd::Node*> seen{root.get()};
+  while (!todo.empty()) {
+    torch::autograd::Node* node = todo.back();
+    todo.pop_back();
+    const auto s = node->stream();
+    if (s && s->id() == none)
+      refuse(std::string(what) + ": a captured backward pass cannot reach into an eager graph of the default stream: run the " +
+             "warm-up on the capture's own stream and release its graph, or capture under torch.no_grad()");
+    for (const auto& edge : node->next_edges())
+      if (edge.function && seen.insert(edge.function.get()).second) todo.push_back(edge.function.get());
+  }
 }
 
 // int32 / int64 numbers on t's device, contiguous; host tensors are uploaded

@@ -1051,3 +1051,55 @@ def test_forward_mode_tangents_are_refused():
         want = ops.layernorm_rows(x)
         assert torch.equal(ops.layernorm_rows(fw.unpack_dual(held).primal), want)
     assert torch.equal(ops.layernorm_rows(held), want)                    # the level is gone, and the tangent with it
+
+
+def test_capture_refuses_eager_leaves_behind_recorded_operations():
+    """The leaf of a live eager graph of the default stream, reached through operations that the capture itself records: refused
+    by the forward call (no backward pass is made here). Once the eager graph is gone the same chains are captured, and replay
+    the eager bits."""
+    from mmssl_amd import ops
+    from mmssl_amd._lib import MmsslError
+    q = gen(91)
+    w = torch.randn(50, 64, generator=q).to(DEV).requires_grad_(True)
+    v = torch.randn(64, generator=q).to(DEV).requires_grad_(True)
+    rows = torch.randn(20, 64, generator=q).to(DEV)
+    idx = torch.arange(20, device=DEV)
+    chains = [("one operation", lambda: ops.embed_rows(w.to(torch.bfloat16), idx)),
+              ("a parameter", lambda: ops.layernorm_rows(rows, v * 2.0)),
+              ("a product", lambda: ops.logprobs_rows(rows @ w.t(), idx)[0]),
+              ("several", lambda: ops.layernorm_rows(((rows + 1.0) * (w[:20] - 2.0)).exp().tanh())),
+              ("an operator of this package", lambda: ops.layernorm_rows(ops.embed_rows(w * 1.0, idx)))]
+    eager = ops.layernorm_rows(ops.embed_rows(w, idx), v)                # kept: holds the accumulators of w and v
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+
+    def captured(fn):
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
+            out = fn()
+        return g, out
+
+    for name, fn in chains:
+        print(name, flush=True)
+        with pytest.raises(MmsslError, match="eager graph of the default stream"):
+            captured(fn)
+    del eager
+    for name, fn in chains:
+        print(name, flush=True)
+        with torch.no_grad():
+            want = fn()
+        g, out = captured(lambda: fn().detach())
+        for _ in range(3):
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), name
+    # eagerly, also on a stream of its own, nothing is refused
+    keep = [fn() for _, fn in chains]
+    with torch.cuda.stream(stream):
+        stream.wait_stream(torch.cuda.default_stream())
+        keep += [fn() for _, fn in chains]
+    torch.cuda.synchronize()
+    for a, b in zip(keep[:5], keep[5:]):
+        assert torch.equal(a, b)
