@@ -105,6 +105,9 @@ std::string shape_of(at::IntArrayRef s) {
   return r + "]";
 }
 
+// The kernels read memory as it is: a lazily negated view (the imaginary part of a conjugate) is written out first.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // t as [rows, d] with unit column stride (a view where the strides allow it) and its row pitch
 struct Rows {
   Tensor t;
@@ -199,7 +202,7 @@ struct EmbedRows : torch::autograd::Function<EmbedRows> {
     const Tensor idx = ctx->get_saved_variables()[0];
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
     const int64_t rows = cfg[0], d = cfg[1];
-    const Rows g = rows_of(grads[0]);
+    const Rows g = rows_of(plain(grads[0]));
     const c10::DeviceGuard guard(g.t.device());
     Tensor grad = at::empty({rows, d}, g.t.options());
     const size_t nb = CALL(mmssl_embed_rows_bwd_workspace_bytes)(rows, (int)d, idx.numel());
@@ -213,8 +216,9 @@ struct EmbedRows : torch::autograd::Function<EmbedRows> {
   }
 };
 
-Tensor embed_rows(const Tensor& table, const Tensor& idx_, double scale, std::optional<int64_t> padding_idx) {
-  typed(table, "table");
+Tensor embed_rows(const Tensor& table_, const Tensor& idx_, double scale, std::optional<int64_t> padding_idx) {
+  typed(table_, "table");
+  const Tensor table = plain(table_);
   if (table.dim() != 2 || table.size(1) < 1 || (table.size(1) > 1 && table.stride(1) != 1))
     refuse("embed_rows: table must be [rows, d] with unit column stride");
   fits_int(table.size(1), "embed_rows");
@@ -260,7 +264,7 @@ struct LayerNormRows : torch::autograd::Function<LayerNormRows> {
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
     const auto pt = (at::ScalarType)cfg[0];
     const c10::DeviceGuard guard(X.device());
-    const Rows x = rows_of(X), g = rows_of(grads[0]);
+    const Rows x = rows_of(X), g = rows_of(plain(grads[0]));
     Tensor gx, gw, gb, ws;
     if (ctx->needs_input_grad(0)) gx = at::empty(X.sizes(), X.options());
     const int edge_b = w.defined() ? 2 : 1;
@@ -280,8 +284,9 @@ struct LayerNormRows : torch::autograd::Function<LayerNormRows> {
   }
 };
 
-Tensor layernorm_rows(const Tensor& X, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
-  typed(X, "X");
+Tensor layernorm_rows(const Tensor& X_, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+  typed(X_, "X");
+  const Tensor X = plain(X_);
   if (X.dim() < 1 || X.size(-1) < 1) refuse("layernorm_rows: X must be [..., d] with d >= 1");
   fits_int(X.size(-1), "layernorm_rows");
   if (!(eps >= 0.0 && eps <= 3.0e38)) refuse("layernorm_rows: eps must be a finite number >= 0, got " + std::to_string(eps));
@@ -293,7 +298,7 @@ Tensor layernorm_rows(const Tensor& X, const std::optional<Tensor>& weight, cons
       refuse(std::string("layernorm_rows: ") + name + " must be [" + std::to_string(X.size(-1)) + "], got " + shape_of(p->sizes()));
     if (p->scalar_type() != X.scalar_type() && p->scalar_type() != at::kFloat)
       refuse(std::string("layernorm_rows: ") + name + " must be of X's type or float32");
-    return p->contiguous();
+    return plain(*p).contiguous();
   };
   const Tensor w = param(weight, "weight"), b = param(bias, "bias");
   if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
@@ -360,7 +365,7 @@ struct LogprobsRows : torch::autograd::Function<LogprobsRows> {
     const c10::DeviceGuard guard(X.device());
     const Rows x = rows_of(X);
     for (Tensor* g : {&gl, &ge, &gt})
-      if (g->defined()) *g = g->contiguous();
+      if (g->defined()) *g = plain(*g).contiguous();
     Tensor gx = at::empty(X.sizes(), X.options());
     check(CALL(mmssl_logprobs_rows_bwd)(x.t.data_ptr(), x.ld, dtype_code(X.scalar_type()), x.rows, x.d, target.data_ptr(),
                                         (int)target.element_size(), cfg[1], (int)cfg[0],
@@ -375,9 +380,10 @@ struct LogprobsRows : torch::autograd::Function<LogprobsRows> {
   }
 };
 
-py::tuple logprobs_rows(const Tensor& X, const Tensor& target_, int64_t k, double temperature, int64_t ignore) {
+py::tuple logprobs_rows(const Tensor& X_, const Tensor& target_, int64_t k, double temperature, int64_t ignore) {
   constexpr int64_t kMost = 128;
-  typed(X, "X");
+  typed(X_, "X");
+  const Tensor X = plain(X_);
   if (X.dim() < 1 || X.size(-1) < 1) refuse("logprobs_rows: X must be [..., n] with n >= 1");
   if (k < 0 || k > kMost || k > X.size(-1))
     refuse("logprobs_rows: 0 <= k <= min(" + std::to_string(kMost) + ", n) expected, got " + std::to_string(k));
@@ -449,6 +455,8 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, double eps,
       refuse("clip_grads: " + std::to_string(out->size()) + " outputs for " + std::to_string(grads.size()) + " gradients");
     o = list_of(*out, "clip_grads: out", dev);
     if (o.numel != l.numel || o.dtype != l.dtype) refuse("clip_grads: out must match the gradients' types and sizes");
+    for (size_t i = 0; i < grads.size(); ++i)          // (in place, and for the norm, a lazy sign makes no difference)
+      if ((*out)[i].is_neg() != grads[i].is_neg()) refuse("clip_grads: out and a lazily negated gradient differ in sign");
   } else {
     o = l;
   }

@@ -1103,3 +1103,41 @@ def test_capture_refuses_eager_leaves_behind_recorded_operations():
     torch.cuda.synchronize()
     for a, b in zip(keep[:5], keep[5:]):
         assert torch.equal(a, b)
+
+
+def test_lazily_negated_views_count_as_what_they_show():
+    """The imaginary part of a conjugate holds its values with the other sign in memory: one column (whose strides need no copy),
+    several, as an operand, as a parameter, as an incoming gradient, in lists."""
+    from mmssl_amd import ops, optim
+    from mmssl_amd._lib import MmsslError
+    q = gen(95)
+    idx = torch.arange(6, device=DEV)
+
+    def both(*shape):
+        v = torch.randn(shape, dtype=torch.complex64, generator=q).to(DEV).conj().imag
+        assert v.is_neg()
+        return v, v.resolve_neg().contiguous()
+
+    for d in (1, 5):
+        (x, y), (g, h), (w, u) = both(6, d), both(6, d), both(d)
+        for fn in (lambda v, w: ops.embed_rows(v if d == 1 else v.contiguous(), idx), lambda v, w: ops.layernorm_rows(v, w, w),
+                   lambda v, w: ops.layernorm_rows(y, w), lambda v, w: ops.logprobs_rows(v, idx.clamp(max=d - 1), k=1)[2]):
+            assert torch.equal(fn(x, w), fn(y, u)), d
+        for fn in (lambda v, w: ops.embed_rows(v, idx), lambda v, w: ops.layernorm_rows(v, w)):
+            leaf, lw = y.clone().requires_grad_(True), u.clone().requires_grad_(True)
+            out = fn(leaf, lw)
+            for a, b in zip(torch.autograd.grad(out, (leaf, lw), g, allow_unused=True, retain_graph=True),
+                            torch.autograd.grad(out, (leaf, lw), h, allow_unused=True)):
+                assert (a is None and b is None) or torch.equal(a, b), d
+    (x, y), (g, h) = both(6, 300), both(6)
+    leaf = y.clone().requires_grad_(True)
+    out = ops.logprobs_rows(leaf, idx)[0]
+    assert torch.equal(torch.autograd.grad(out, leaf, g, retain_graph=True)[0], torch.autograd.grad(out, leaf, h)[0])
+    (a, b) = both(1)
+    assert a.is_contiguous()
+    assert torch.equal(optim.grad_norm([a]), optim.grad_norm([b]))
+    with pytest.raises(MmsslError):
+        optim.clip_grads([a], 0.25, out=[torch.zeros_like(b)])
+    optim.clip_grads([a], 0.25)
+    optim.clip_grads([b], 0.25)
+    assert torch.equal(a, b)
