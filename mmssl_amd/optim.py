@@ -194,7 +194,8 @@ def _grads(grads):
 
 def grad_norm(grads):
     """The 2-norm of all elements of a list of gradients together (fp32 / bf16 / fp16, mixed, any sizes) as a 0-dim fp32 device
-    tensor: one launch over all of them and a small one, 64-bit sums in a fixed order, nothing read back."""
+    tensor: one launch over all of them and a small one, 64-bit sums in a fixed order, nothing read back. Not differentiable:
+    tensors that require grad are refused outside torch.no_grad()."""
     return _lib.binding().grad_norm(_grads(grads))
 
 
@@ -202,7 +203,8 @@ def clip_grads(grads, max_norm, out=None):
     """Scale a list of gradients down to the global norm `max_norm` (times min(1, max_norm / (norm + 1e-6))) and return the norm
     they had, a 0-dim fp32 device tensor. `out`: where the scaled gradients go, one tensor of the same type and number of
     elements per gradient (default: the gradients themselves). What is written may overlap nothing else. The factor never
-    leaves the device; a NaN among the gradients makes all of them NaN, an infinite norm the finite ones 0."""
+    leaves the device; a NaN among the gradients makes all of them NaN, an infinite norm the finite ones 0. Not differentiable:
+    tensors that require grad (parameters in place of their gradients, say) are refused outside torch.no_grad()."""
     return _lib.binding().clip_grads(_grads(grads), max_norm, CLIP_EPS,
                                      None if out is None else _grads(out))
 
@@ -215,8 +217,8 @@ def clip_grad_norm(parameters, max_norm):
     if not grads:
         raise _lib.MmsslError("clip_grad_norm: no parameter has a gradient")
     flat = [g if g.layout != torch.strided or g.is_contiguous() else g.contiguous() for g in grads]
-    norm = clip_grads(flat, max_norm)
-    with torch.no_grad():
+    with torch.no_grad():                       # gradients of a create_graph=True pass require grad themselves
+        norm = clip_grads(flat, max_norm)
         for g, f in zip(grads, flat):
             if f is not g:
                 g.copy_(f)

@@ -1141,3 +1141,32 @@ def test_lazily_negated_views_count_as_what_they_show():
     optim.clip_grads([a], 0.25)
     optim.clip_grads([b], 0.25)
     assert torch.equal(a, b)
+
+
+def test_gradient_lists_that_require_grad():
+    """Norms and clipping are not recorded: what requires grad is refused while a graph is recorded, before anything is written.
+    Without recording, and for the .grad of a create_graph=True pass, they run."""
+    from mmssl_amd import optim
+    from mmssl_amd._lib import MmsslError
+    p = torch.nn.Parameter(torch.full((16,), 2.0, device=DEV))
+    h = p * 3.0
+    plain = torch.ones(16, device=DEV)
+    for fn in (lambda: optim.grad_norm([p]), lambda: optim.grad_norm([plain, h]), lambda: optim.clip_grads([p], 1.0),
+               lambda: optim.clip_grads([plain, h], 1.0), lambda: optim.clip_grads([plain], 1.0, out=[p]),
+               lambda: optim.clip_grads([h], 1.0, out=[plain])):
+        with pytest.raises(MmsslError, match="not differentiable"):
+            fn()
+    assert bool((p == 2.0).all()) and bool((h == 6.0).all()) and bool((plain == 1.0).all())
+    with torch.no_grad():
+        want = (16 * 4.0 + 16 * 36.0) ** 0.5        # no fp32 number: the result is rounded once, half a step off at most
+        assert abs(float(optim.grad_norm([p, h])) - want) <= want * 2.0 ** -24
+        assert float(optim.clip_grads([p], 4.0)) == 8.0
+    assert float((p.detach() - 1.0).abs().max()) <= 1e-6
+    loss = (p ** 3).sum()
+    loss.backward(create_graph=True)
+    assert p.grad.requires_grad
+    want = p.grad.detach() / 12.0                                          # gradients of 3, sixteen of them: norm 12
+    norm = optim.clip_grad_norm([p], 1.0)
+    assert not norm.requires_grad and abs(float(norm) - 12.0) <= 1e-4
+    assert float((p.grad.detach() - want).abs().max()) <= 1e-5
+    p.grad = None
