@@ -211,12 +211,19 @@ def clip_grads(grads, max_norm, out=None):
 
 def clip_grad_norm(parameters, max_norm):
     """clip_grads over the `.grad` of the parameters that have one, in place (what a training loop calls between backward and
-    FusedAdamW.step). A gradient that is not contiguous is scaled through a contiguous copy."""
+    FusedAdamW.step). A gradient that is not contiguous is scaled through a contiguous copy. One that several parameters share
+    counts for each of them in the norm and is scaled once; gradients that overlap without being the same tensor are refused."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         raise _lib.MmsslError("clip_grad_norm: no parameter has a gradient")
     flat = [g if g.layout != torch.strided or g.is_contiguous() else g.contiguous() for g in grads]
+    if len(set(map(id, grads))) < len(grads):
+        seen = set()
+        for i, g in enumerate(grads):
+            if id(g) in seen and flat[i] is g and g.layout == torch.strided:
+                flat[i] = g.detach().clone()
+            seen.add(id(g))
     with torch.no_grad():                       # gradients of a create_graph=True pass require grad themselves
         norm = clip_grads(flat, max_norm)
         for g, f in zip(grads, flat):

@@ -1170,3 +1170,30 @@ def test_gradient_lists_that_require_grad():
     assert not norm.requires_grad and abs(float(norm) - 12.0) <= 1e-4
     assert float((p.grad.detach() - want).abs().max()) <= 1e-5
     p.grad = None
+
+
+def test_parameters_that_share_a_gradient():
+    """Two parameters with one .grad, contiguous and not, and the same parameter twice: counted each time, scaled once."""
+    from mmssl_amd import optim
+    from mmssl_amd._lib import MmsslError
+    q = gen(97)
+    for make in (lambda: torch.randn(30, 50, generator=q).to(DEV), lambda: torch.randn(50, 30, generator=q).to(DEV).t()):
+        a, b, c = (torch.nn.Parameter(torch.zeros(30, 50, device=DEV)) for _ in range(3))
+        a.grad, c.grad = make(), torch.randn(30, 50, generator=q).to(DEV)
+        b.grad = a.grad
+        was, other = a.grad.double(), c.grad.double()
+        for given, times in (([a, b, c], 2), ([a, c, a, b], 3)):
+            assert b.grad is a.grad
+            total = float((times * (was ** 2).sum() + (other ** 2).sum()) ** 0.5)
+            norm = optim.clip_grad_norm(given, total / 2)
+            assert abs(float(norm) - total) <= total * (2.0 ** -24 + 1e-12)
+            factor = total / 2 / (total + 1e-6)
+            for p, w in ((a, was), (c, other)):
+                # the factor is rounded to 32 bits, so is the product
+                within(p.grad, w * factor, (w * factor).abs().cpu() * 2.0 ** -22 + 1e-30, "grad")
+            was, other = a.grad.double(), c.grad.double()
+    whole = torch.randn(40, device=DEV)
+    a, b = (torch.nn.Parameter(torch.zeros(30, device=DEV)) for _ in range(2))
+    a.grad, b.grad = whole[:30], whole[10:]
+    with pytest.raises(MmsslError, match="overlap"):
+        optim.clip_grad_norm([a, b], 1.0)
