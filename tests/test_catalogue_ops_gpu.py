@@ -1069,9 +1069,13 @@ def test_capture_refuses_eager_leaves_behind_recorded_operations():
               ("a product", lambda: ops.logprobs_rows(rows @ w.t(), idx)[0]),
               ("several", lambda: ops.layernorm_rows(((rows + 1.0) * (w[:20] - 2.0)).exp().tanh())),
               ("an operator of this package", lambda: ops.layernorm_rows(ops.embed_rows(w * 1.0, idx)))]
-    eager = ops.layernorm_rows(ops.embed_rows(w, idx), v)                # kept: holds the accumulators of w and v
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(stream):        # a library's first product sets the library up, which no capture holds
+        for _, fn in chains:
+            fn()
+    torch.cuda.synchronize()
+    eager = ops.layernorm_rows(ops.embed_rows(w, idx), v)                # kept: holds the accumulators of w and v
 
     def captured(fn):
         g = torch.cuda.CUDAGraph()
