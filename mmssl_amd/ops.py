@@ -1425,6 +1425,14 @@ def _numbers(idx):
     return idx if idx.numel() else idx.to(torch.int64)
 
 
+def _factor(v, name):
+    """A plain number; one with a gradient of its own would lose it in the conversion."""
+    if isinstance(v, torch.Tensor) and v.requires_grad and torch.is_grad_enabled():
+        raise _lib.MmsslError("%s is a plain number: there is no gradient for it. Multiply outside, or pass float(%s)"
+                              % (name, name))
+    return v
+
+
 def embed_rows(table, idx, scale=1.0, padding_idx=None):
     """scale * table[idx]: rows of an embedding table [rows, d] for tokens of any shape (int64 or int32), fp32 / bf16 / fp16,
     rounded once. `padding_idx`: tokens of this number (in the table or not, e.g. the -1 that topk_rows pads with) give rows
@@ -1432,7 +1440,7 @@ def embed_rows(table, idx, scale=1.0, padding_idx=None):
     adds equal tokens in the order of their places with fp32 sums (the same call gives the same bits); padding and tokens
     outside the table add nothing."""
     _given(table, "table")
-    return _lib.binding().embed_rows(table, _numbers(idx), scale, padding_idx)
+    return _lib.binding().embed_rows(table, _numbers(idx), _factor(scale, "scale"), padding_idx)
 
 
 def layernorm_rows(X, weight=None, bias=None, eps=1e-5):
@@ -1440,7 +1448,7 @@ def layernorm_rows(X, weight=None, bias=None, eps=1e-5):
     and variances, rounded once. `weight` / `bias`: [d] tensors of X's type or fp32 (both of one type), or None.
     Differentiable in X, weight and bias; the parameters' sums over the rows are fp32 in a fixed order."""
     _given(X, "X")
-    return _lib.binding().layernorm_rows(X, weight, bias, eps)
+    return _lib.binding().layernorm_rows(X, weight, bias, _factor(eps, "eps"))
 
 
 def logprobs_rows(X, target, k=0, temperature=1.0, ignore_index=-100):
@@ -1453,4 +1461,4 @@ def logprobs_rows(X, target, k=0, temperature=1.0, ignore_index=-100):
     and entropy NaN. Differentiable in X through logp, entropy and top_logp. Up to 2^24 - 1 rows of up to 2048 columns (of longer
     ones as many fewer)."""
     _given(X, "X")
-    return _lib.binding().logprobs_rows(X, _numbers(target), k, temperature, ignore_index)
+    return _lib.binding().logprobs_rows(X, _numbers(target), k, _factor(temperature, "temperature"), ignore_index)

@@ -1201,3 +1201,21 @@ def test_parameters_that_share_a_gradient():
     a.grad, b.grad = whole[:30], whole[10:]
     with pytest.raises(MmsslError, match="overlap"):
         optim.clip_grad_norm([a, b], 1.0)
+
+
+def test_factors_that_require_grad_are_refused():
+    from mmssl_amd import ops
+    from mmssl_amd._lib import MmsslError
+    x = torch.randn(6, 40, generator=gen(99)).to(DEV)
+    idx = torch.arange(6, device=DEV)
+    two = torch.tensor(2.0, device=DEV, requires_grad=True)
+    calls = [lambda v: ops.embed_rows(x, idx, scale=v), lambda v: ops.layernorm_rows(x, eps=v),
+             lambda v: ops.logprobs_rows(x, idx, temperature=v)[0]]
+    for fn in calls:
+        want = fn(2.0)
+        for v in (two, two * 1.0):
+            with pytest.raises(MmsslError, match="plain number"):
+                fn(v)
+            with torch.no_grad():
+                assert torch.equal(fn(v), want)
+        assert torch.equal(fn(two.detach()), want)
