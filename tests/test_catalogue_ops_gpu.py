@@ -1219,3 +1219,76 @@ def test_factors_that_require_grad_are_refused():
             with torch.no_grad():
                 assert torch.equal(fn(v), want)
         assert torch.equal(fn(two.detach()), want)
+
+
+def popular_places(kind, n, rows, q):
+    """Tokens of n places: evenly spread, one with all or half of them, steeply falling, the first and the last."""
+    u = torch.rand(n, generator=q, device=DEV)
+    return {"even": lambda: (rows * u).long().clamp_(max=rows - 1), "one": lambda: torch.full((n,), rows // 2, device=DEV),
+            "half": lambda: torch.where(u < 0.5, torch.full_like(u, 7), rows * u).long().clamp_(max=rows - 1),
+            "steep": lambda: (rows * u ** 6).long().clamp_(max=rows - 1),
+            "two": lambda: torch.where(u < 0.4, 0, rows - 1)}[kind]().long()
+
+
+def whole_sums(idx, whole, rows):
+    """Sums of whole numbers (int64) over the places of each token, exactly: differences of running sums along the sorted list."""
+    key, order = torch.sort(idx)
+    run = torch.cat([torch.zeros_like(whole[:1]), whole[order].cumsum(0)])
+    at = torch.searchsorted(key, torch.arange(rows + 1, device=DEV))
+    return run[at[1:]] - run[at[:-1]]
+
+
+@pytest.mark.parametrize("kind", ["even", "one", "half", "steep", "two"])
+@pytest.mark.parametrize("n", [32767, 32768, 524287, 524288, 600011])
+def test_embed_gradient_where_chunks_change_length(n, kind):
+    """Lists around the lengths at which a chunk goes from 8 to 16 and from 16 to 64 places. Whole numbers: every sum stays below 2^24
+    (at most 600011 terms of at most 8), so fp32 holds it and each sum on the way exactly, in any order, and the results
+    are equal; a half type rounds that once."""
+    from mmssl_amd import ops
+    rows = 3001
+    q = torch.Generator(device=DEV).manual_seed(n)
+    idx = popular_places(kind, n, rows, q)
+    for d, t in ((8, torch.float32), (64, torch.bfloat16), (300, torch.float32), (65, torch.float16)):
+        whole = torch.randint(-8, 9, (n, d), generator=q, device=DEV)
+        w = torch.zeros(rows, d, device=DEV, dtype=t, requires_grad=True)
+        (a,) = torch.autograd.grad(ops.embed_rows(w, idx, scale=0.5), w, whole.to(t))
+        assert torch.equal(a, (whole_sums(idx, whole, rows).double() * 0.5).to(t)), (d, t)
+
+
+@pytest.mark.parametrize("kind", ["even", "one", "half", "steep", "two"])
+@pytest.mark.parametrize("n", [300001, 524287, 524288])
+def test_embed_gradient_of_long_lists_within_the_chain_of_its_sums(n, kind):
+    """Numbers with 20 bits behind the point, whose sums fp32 has to round. A term passes the sum of its chunk (16 places below
+    2^19 of them, 64 from there on), then, over more than 16 chunks, the sum of one of the block's lane groups (each takes
+    every so-manyth chunk), the groups' sum and the first chunk's part: off by 2^-24 of the magnitudes for each."""
+    from mmssl_amd import ops
+    rows = 3001
+    q = torch.Generator(device=DEV).manual_seed(n + 1)
+    idx = popular_places(kind, n, rows, q)
+    chunk = 64 if n >= 1 << 19 else 16
+    chunks = -(-n // chunk)
+    for d, lanes in ((20, 8), (64, 16), (300, 64)):
+        groups = 256 // lanes
+        chain = chunk + max(16, -(-chunks // groups)) + groups + 1
+        whole = (torch.randn(n, d, generator=q, device=DEV) * 2 ** 20).round().clamp_(-(2 ** 23), 2 ** 23).long()
+        w = torch.zeros(rows, d, device=DEV, requires_grad=True)
+        (a,) = torch.autograd.grad(ops.embed_rows(w, idx), w, whole.float() / 2 ** 20)
+        want, size = whole_sums(idx, whole, rows).double() / 2 ** 20, whole_sums(idx, whole.abs(), rows).double() / 2 ** 20
+        assert bool(((a.double() - want).abs() <= chain * 2.0 ** -24 * size).all()), d
+
+
+def test_long_gradient_lists_clip_every_element():
+    """Lists of more chunks than a block looks ahead, as above, every element against its own value, into outputs that hold
+    something else before."""
+    from mmssl_amd import optim
+    sizes = [5_770_000 + 37 * i for i in range(96)] + [1_000_003]
+    grads = [torch.full((n,), 1.0 + i % 3, device=DEV, dtype=torch.bfloat16) for i, n in enumerate(sizes)]
+    for i, g in enumerate(grads):
+        g[-1] = 200.0 + i                                                 # (rounded by the type)
+    norm = sum(int(g[-1]) ** 2 + (n - 1) * (1 + i % 3) ** 2 for i, (n, g) in enumerate(zip(sizes, grads))) ** 0.5
+    out = [torch.full_like(g, float("nan")) for g in grads]
+    optim.clip_grads(grads, norm / 256, out=out)
+    for i, (g, o) in enumerate(zip(grads, out)):
+        # the factor is 2^-8 up to a few half steps of 32 bits, and the product's nearest bf16 number is the value's 2^-8 fold,
+        # which bf16 holds: no element is off at all
+        assert torch.equal(o.float() * 256, g.float()), i
