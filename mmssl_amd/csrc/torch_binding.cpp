@@ -412,12 +412,15 @@ GradList list_of(const std::vector<Tensor>& ts, const char* what, c10::Device de
   l.at.reserve(ts.size());
   l.numel.reserve(ts.size());
   l.dtype.reserve(ts.size());
+  const bool recording = at::GradMode::is_enabled();
   for (const Tensor& t : ts) {
     if (!t.defined() || t.layout() != at::kStrided) refuse(std::string(what) + ": dense tensors expected");
-    no_tangent(t, what);
-    // nothing of this is recorded: a norm would be a constant of its backward pass, a leaf be written behind autograd's back
-    if (t.requires_grad() && at::GradMode::is_enabled())
-      refuse(std::string(what) + ": not differentiable; detach the tensors or call it under torch.no_grad()");
+    if (t.unsafeGetTensorImpl()->autograd_meta()) {      // plain data has neither
+      no_tangent(t, what);
+      // nothing of this is recorded: a norm would be a constant of its backward pass, a leaf be written behind autograd's back
+      if (recording && t.requires_grad())
+        refuse(std::string(what) + ": not differentiable; detach the tensors or call it under torch.no_grad()");
+    }
     if (!t.is_cuda() || t.device() != dev)
       refuse(std::string(what) + ": gradients must be on one CUDA (HIP) device: this package has no CPU path");
     const int c = dtype_code(t.scalar_type());

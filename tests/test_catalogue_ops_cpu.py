@@ -134,3 +134,26 @@ def test_missing_binding_fails_loudly():
             "    print('LOUD', 'no fallback' in str(e))\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
     assert "LOUD True" in r.stdout, r.stdout + r.stderr
+
+
+def test_what_derivatives_would_lose_is_refused_before_the_device_is_looked_at():
+    """Factors and gradient lists that require grad, lists with forward-mode tangents: host tensors do, the reason given is theirs."""
+    from torch.autograd import forward_ad as fw
+    from mmssl_amd import ops, optim
+    from mmssl_amd._lib import MmsslError
+    x, idx = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    two = torch.tensor(2.0, requires_grad=True)
+    for fn in (lambda: ops.embed_rows(x, idx, scale=two), lambda: ops.layernorm_rows(x, eps=two * 1.0),
+               lambda: ops.logprobs_rows(x, idx, temperature=two)):
+        with pytest.raises(MmsslError, match="plain number"):
+            fn()
+    p = torch.nn.Parameter(torch.ones(4))
+    for fn in (lambda: optim.grad_norm([p]), lambda: optim.clip_grads([p * 2.0], 1.0), lambda: optim.grad_norm(p)):
+        with pytest.raises(MmsslError, match="not differentiable"):
+            fn()
+    with fw.dual_level():
+        dual = fw.make_dual(torch.ones(4), torch.ones(4))
+        for fn in (lambda: optim.grad_norm([dual]), lambda: optim.clip_grads([dual], 1.0)):
+            with pytest.raises(MmsslError, match="forward-mode"):
+                fn()
+    assert bool((p == 1.0).all())
