@@ -2,14 +2,14 @@
 //
 //   out[i, :] = scale * table[idx[i], :]            gW[v, :] = scale * sum over i with idx[i] = v of g[i, :]
 //
-// The gradient adds the rows of equal tokens in the order of their places: the places are sorted by token (stable), the
-// sorted list is cut into equal chunks, a lane group walks a chunk and keeps the running sum of the token it is at. A sum
-// that lies inside a chunk is written at once; one that crosses a chunk's border leaves a partial row that a last launch
-// joins in the chunks' order. No float atomics: the same call gives the same bits.
+// The gradient adds the rows of equal tokens in a fixed order: the places are sorted by token (stable), the sorted list is cut
+// into equal chunks, a lane group walks a chunk and keeps the running sum of the token it is at. A sum that lies inside a
+// chunk is written at once; one that crosses a chunk's border leaves a partial row that a last launch joins, in the
+// chunks' order or, over more than 16 of them, lane group by lane group. No float atomics: the same call gives the same bits.
 //
-// Both directions are bound by memory where they are large: 1 000 003 places of 1 M x 128 bf16 look up in 80 us (457 MB moved, 5.7
-// TB/s), are summed in 124 us (590 MB, 4.8 TB/s, rows at random) after three radix passes of 22 us each (latency: the pairs are 8
-// MB and come from the caches) and joined in 12. 1024 rows of 64 fp32 look up in 3.4 us, a launch.
+// Both directions are bound by memory where they are large: 1 000 003 places of 1 M x 128 bf16 look up in 83 us (457 MB moved, 5.5
+// TB/s), are summed in 127 us (590 MB, 4.6 TB/s, rows at random) after three radix passes of 23 us each (latency: the pairs are 8
+// MB and come from the caches) and joined in 13. 1024 rows of 64 fp32 look up in 3.5 us, a launch.
 #include <algorithm>
 
 #include "typed.hpp"
@@ -481,7 +481,9 @@ Plan plan_for(int64_t rows, int d, int64_t n) {
   p.per = (tiles + kSortBlocks - 1) / kSortBlocks * kSortThreads;
   p.blocks = n ? (n + p.per - 1) / p.per : 0;
   // places of a chunk: longer ones leave fewer partial rows, shorter ones more lanes at work. The whole gradient into 18357 x 64
-  // fp32 with 8 / 16 / 64: 8192 places 25 / 25 / 37 us, 51200 32 / 32 / 44, 524288 78 / 71 / 58.
+  // fp32 with 8 / 16 / 64: 8192 places 25 / 25 / 37 us, 51200 32 / 32 / 44, 524288 78 / 71 / 58. At other widths: 8 columns, 8192
+  // places 29 / 30 / 41, 524287 88 / 83 / 81; 1024 columns 38 / 37 / 49 and 674 / 580 / 510 (65536 places 107 / 98 / 93: wide rows would
+  // gain up to 12 % from 64 earlier, the rule does not look at the width).
   p.chunk = n >= (1 << 19) ? 64 : n >= (1 << 15) ? 16 : 8;
   p.chunks = (n + p.chunk - 1) / p.chunk;
   p.npad = (n + 15) / 16 * 16;

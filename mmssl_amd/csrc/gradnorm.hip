@@ -8,8 +8,8 @@
 // blocks share the tensors' chunks evenly and leave one partial sum each. The
 // sums are in 64 bits: the square of every fp32 number is representable, nothing overflows or vanishes on the way, and the
 // conversions hide behind the loads. The scaling launch adds the partial sums up again in every block (a few KB out of the
-// cache) instead of waiting for a launch that would do it once, and walks the chunks from the back, where the norm's launch
-// has just left them in the caches.
+// cache) instead of waiting for a launch that would do it once. With a list in the arguments it walks the chunks from the back,
+// where the norm's launch has just left them in the caches; in a longer list each block walks its own run of chunks forwards.
 #include <algorithm>
 
 #include "typed.hpp"

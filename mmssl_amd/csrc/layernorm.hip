@@ -8,8 +8,8 @@
 // are the same for every row, so the weight stays in registers and the weight's gradient adds up there over the rows of a
 // block; the blocks' partial sums meet in a second launch in a fixed order. Rows longer than 16384 are swept from memory.
 //
-// Bound by memory: 65536 x 4096 bf16 forward 200 us (1.07 GB, 5.4 TB/s), backward 302 (1.61 GB, 5.3 TB/s) and 8 for the
-// parameters' sums; 51197 x 256 fp32 21 + 27 + 4 us; 1024 x 64 fp32 3.2, a launch. Rows of 20000 fp32: 3.4 and 2.3 TB/s.
+// Bound by memory: 65536 x 4096 bf16 forward 206 us (1.07 GB, 5.2 TB/s; best of 15 launches 199), backward 317 (1.61 GB, 5.1 TB/s;
+// best 297) and 8 for the parameters' sums; 51197 x 256 fp32 21 + 27 + 4 us; 1024 x 64 fp32 3.2, a launch. Rows of 20000 fp32: 3.4 and 2.3 TB/s.
 #include <algorithm>
 
 #include "typed.hpp"

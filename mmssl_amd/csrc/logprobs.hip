@@ -10,8 +10,8 @@
 // about 2 k candidates, which are ranked by counting.
 // Backward: one read of X, one write of gx.
 //
-// Bound by memory from some ten million scores on: 8192 x 35598 bf16 forward 150 us (583 MB: 3.9 TB/s, with the target's and the
-// join's 5 us), backward 200 us (1.17 GB, 5.8 TB/s). With alternatives by the phases that follow the loads in every block: 1024 x
+// Bound by memory from some ten million scores on: 8192 x 35598 bf16 forward 148 us (583 MB: 3.9 TB/s; best of 15 launches 129) and 5
+// for the join, backward 214 us (1.17 GB, 5.5 TB/s; best 202). With alternatives by the phases that follow the loads in every block: 1024 x
 // 18357 fp32 with 50 of them 27 us (75 MB) and 7 for the join; one row of 1 M columns with 20: 6.5 + 7.3, latency.
 #include <algorithm>
 
@@ -620,8 +620,9 @@ struct Cut {
 };
 
 // Slices of 32 values a thread (with 64, two thirds of the waves fit: 8192 x 35598 bf16 forward 188 -> 150 us, 1024 x 18357 fp32
-// with 50 alternatives 34 -> 28 us); shorter ones where that leaves fewer than 512 blocks. Slices of a row are of equal length,
-// to whole vectors.
+// with 50 alternatives 34 -> 28 us); shorter ones where that leaves fewer than 512 blocks: with 128 / 256 / 512 / 1024 instead, 1 x 1 M
+// fp32 6.6 / 7.1 / 7.2 / 7.2 us and with 20 alternatives 12.3 / 13.5 / 13.6 / 13.4, 64 x 18357 6.6 / 6.6 / 6.7 / 7.3 and 12.2 / 11.3 / 11.9 /
+// 12.2, 200 x 18357 7.2 / 7.1 / 7.1 / 7.4 and 13.6 / 13.6 / 13.7 / 14.5. Slices of a row are of equal length, to whole vectors.
 Cut cut_for(int64_t rows, int64_t cols, int es) {
   const int n = 16 / es, most = 32 / n;
   Cut q{};
@@ -649,7 +650,7 @@ int check_common(int dtype, int64_t rows, int64_t cols, int target_bytes, int k,
   if (!known_dtype(dtype) || rows < 0 || cols < 1 || (target_bytes != 4 && target_bytes != 8) || k < 0) return MMSSL_E_BADARG;
   if (!(temperature > 0.f) || temperature > 3.0e38f || !(1.0f / temperature <= 3.0e38f)) return MMSSL_E_BADARG;
   if (k > kTopMax || k > cols || cols > 0x7ffffff0) return MMSSL_E_UNSUPP;
-  // a row's slices are no shorter than 2048 columns (but for the last), so its pairs are counted in 32 bits
+  // a row has at most ceil(cols / 2048) slices, so its pairs are counted in 32 bits
   if (rows > 0x7fffffff || !launchable(rows * ((cols + 2047) / 2048), kBlock)) return MMSSL_E_UNSUPP;
   return 0;
 }

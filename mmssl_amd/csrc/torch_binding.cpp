@@ -3,8 +3,8 @@
 // interpreter in between. What the GPU does is libmmssl_hip.so's, reached through its C ABI like every other operator; this
 // file launches nothing by itself.
 //
-// Measured on one MI355X host, 200 rows looked up in a 500 x 64 fp32 table: forward 4.1 us (through ctypes 8.3), forward and
-// gradient through torch.autograd.grad 56 us (a Python autograd.Function over ctypes 92; the engine's own share is about 40).
+// Measured on one MI355X host, 200 rows looked up in a 500 x 64 fp32 table: forward 4.5 us (through ctypes 8.3), forward and
+// gradient through torch.autograd.grad 57 us (a Python autograd.Function over ctypes 92; the engine's own share is about 40).
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>

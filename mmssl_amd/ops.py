@@ -1437,8 +1437,8 @@ def embed_rows(table, idx, scale=1.0, padding_idx=None):
     """scale * table[idx]: rows of an embedding table [rows, d] for tokens of any shape (int64 or int32), fp32 / bf16 / fp16,
     rounded once. `padding_idx`: tokens of this number (in the table or not, e.g. the -1 that topk_rows pads with) give rows
     of zeros; any other token outside the table gives a row of NaN. Differentiable in `table`: the dense [rows, d] gradient
-    adds equal tokens in the order of their places with fp32 sums (the same call gives the same bits); padding and tokens
-    outside the table add nothing."""
+    adds equal tokens in a fixed order with fp32 sums (the same call gives the same bits); padding and tokens outside the table
+    add nothing. `scale` is a plain number without a gradient."""
     _given(table, "table")
     return _lib.binding().embed_rows(table, _numbers(idx), _factor(scale, "scale"), padding_idx)
 
