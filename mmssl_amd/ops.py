@@ -1426,8 +1426,9 @@ def _numbers(idx):
 
 
 def _factor(v, name):
-    """A plain number; one with a gradient of its own would lose it in the conversion."""
-    if isinstance(v, torch.Tensor) and v.requires_grad and torch.is_grad_enabled():
+    """A plain number; one with a derivative of its own would lose it in the conversion."""
+    if isinstance(v, torch.Tensor) and (v.requires_grad and torch.is_grad_enabled()
+                                        or torch.autograd.forward_ad.unpack_dual(v).tangent is not None):
         raise _lib.MmsslError("%s is a plain number: there is no gradient for it. Multiply outside, or pass float(%s)"
                               % (name, name))
     return v

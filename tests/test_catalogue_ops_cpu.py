@@ -157,3 +157,20 @@ def test_what_derivatives_would_lose_is_refused_before_the_device_is_looked_at()
             with pytest.raises(MmsslError, match="forward-mode"):
                 fn()
     assert bool((p == 1.0).all())
+
+
+def test_factors_with_tangents_are_refused():
+    from torch.autograd import forward_ad as fw
+    from mmssl_amd import ops
+    from mmssl_amd._lib import MmsslError
+    x, idx = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    with fw.dual_level():
+        two = fw.make_dual(torch.tensor(2.0), torch.tensor(1.0))
+        for fn in (lambda: ops.embed_rows(x, idx, scale=two), lambda: ops.layernorm_rows(x, eps=two),
+                   lambda: ops.logprobs_rows(x, idx, temperature=two)):
+            with pytest.raises(MmsslError, match="plain number"):
+                fn()
+            with torch.no_grad(), pytest.raises(MmsslError, match="plain number"):
+                fn()
+    with pytest.raises(MmsslError, match="no CPU path"):          # outside the level it is a number again
+        ops.embed_rows(x, idx, scale=two)
