@@ -19,7 +19,8 @@ using namespace mmssl;
 namespace {
 
 // Up to here the places are ranked by counting (one launch, quadratic work), above by radix passes. The whole gradient into 18357 x
-// 64 fp32: 4096 places 18 against 21 us, 8192 24 against 23, 16384 35 against 25.
+// 64 fp32: 4096 places 18 against 21 us, 8192 24 against 23, 16384 35 against 25. Other tables, 2048 and 8192 places: 200 rows (one pass
+// instead of two) 16 and 26 against 15 and 19, 18357 x 1024 26 and 38 against 30 and 36, 1 M x 64 (three) 45 and 54 against 56 and 59.
 constexpr int kRankMax = 8192;
 constexpr int kSortThreads = 1024;
 constexpr int kSortBlocks = 256;
